@@ -25,7 +25,9 @@ class DabnnError(RuntimeError):
         self.text = text
 
 
-_p, _i, _z, _f = C.c_void_p, C.c_int, C.c_size_t, C.c_float
+LOGPROBS_MAX_TOP = 64             # DABNN_LOGPROBS_MAX_TOP
+
+_p, _i, _z, _f, _l = C.c_void_p, C.c_int, C.c_size_t, C.c_float, C.c_longlong
 # name -> argtypes; every function returns int unless listed in _RESTYPES
 _SIGNATURES = {
     "dabnn_pack_mat": [_p, _p, _i, _i, _i, _i, _p],
@@ -57,6 +59,9 @@ _SIGNATURES = {
     "dabnn_fconv": [_p, _p, _p, _p] + [_i] * 13 + [_p],
     "dabnn_fconv_maxpool_supported": [_i] * 11,
     "dabnn_fconv_maxpool": [_p, _p, _p, _p, _p, _i, _p, _p] + [_i] * 11 + [_p],
+    "dabnn_fp8_quantize": [_p, _i, _l, _p, _l, _p, _l, _l, _i, _i, _i, _p],
+    "dabnn_fp8_gemm": [_p, _l, _p, _l, _l, _p, _l, _p, _l, _l, _p, _p, _i, _l, _i, _i, _i, _p],
+    "dabnn_logprobs": [_p, _i, _l, _p, _i, _i, _p, _p, _p, _p, _p, _i, _p],
     "dabnn_net_create": [C.POINTER(_p)],
     "dabnn_net_destroy": [_p],
     "dabnn_net_set_flags": [_p, _i, _i, _i],
@@ -67,6 +72,7 @@ _SIGNATURES = {
     "dabnn_net_sync": [_p],
     "dabnn_net_get_blob": [_p, C.c_char_p, C.POINTER(_i), C.POINTER(_p), _p, _z],
     "dabnn_net_get_blob_bits": [_p, C.c_char_p, C.POINTER(_i), C.POINTER(_p), _p, _z],
+    "dabnn_net_logprobs": [_p, C.c_char_p, _p, _p, _p, _p, _p, _p, _i],
     "dabnn_net_output_name": [_p, _i],
     "dabnn_net_stream": [_p],
     "dabnn_net_stats": [_p, C.POINTER(_i), C.POINTER(_z)],

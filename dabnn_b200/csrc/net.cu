@@ -133,6 +133,9 @@ struct NetImpl {
     std::vector<std::string> time_names;
     std::vector<float> time_ms;
 
+    unsigned char* score = nullptr;   // labels and results of dabnn_net_logprobs on the device
+    size_t score_bytes = 0;
+
     std::map<std::string, int> bit_names;   // outputs of Binarize layers: blob whose packed sign bits they name
     int* status_words[3] = {nullptr, nullptr, nullptr};   // device addresses of the kernels' status words
     volatile int* status_host = nullptr;                  // mapped pinned word written by status_gather_kernel
@@ -154,6 +157,7 @@ struct NetImpl {
         if (weights) cudaFree(weights);
         if (expanded) cudaFree(expanded);
         if (remainders) cudaFree(remainders);
+        if (score) cudaFree(score);
         if (stream) cudaStreamDestroy(stream);
     }
 
@@ -1170,6 +1174,54 @@ extern "C" int dabnn_net_get_blob_bits(dabnn_net* net, const char* name, int dim
         return n.check_status();
     }
     return DABNN_OK;
+}
+extern "C" int dabnn_net_logprobs(dabnn_net* net, const char* name, const int64_t* labels, float* label_logprob, int64_t* label_rank,
+                                  float* entropy, float* top_logprob, int64_t* top_index, int top) {
+    int dims[4];
+    const float* logits = nullptr;
+    int rc = dabnn_net_get_blob(net, name, dims, &logits, nullptr, 0);
+    if (rc) return rc;
+    NetImpl& n = net->impl;
+    DABNN_REQUIRE(n.cur_batch > 0, DABNN_ERR_STATE, "logprobs: the net has not been run");
+    DABNN_REQUIRE((long long)dims[0] * dims[1] * dims[2] <= INT_MAX, DABNN_ERR_SHAPE, "logprobs: too many rows");
+    DABNN_REQUIRE(top >= 0 && top <= DABNN_LOGPROBS_MAX_TOP && top <= dims[3], DABNN_ERR_ARG, "logprobs: top must be between 0 and the smaller of 64 and the classes");
+    const size_t rows = (size_t)dims[0] * dims[1] * dims[2], tops = rows * top;
+    // 8-byte values first: labels, rank, top index | label log probability, entropy, top log probability
+    const size_t rank_at = rows * 8, index_at = rank_at + rows * 8, lp_at = index_at + tops * 8, entropy_at = lp_at + rows * 4,
+                 top_at = entropy_at + rows * 4, bytes = top_at + tops * 4;
+    DABNN_CUDA_OK(cudaSetDevice(n.device));
+    try {
+        if (bytes > n.score_bytes) {   // the last call waited for its results: the old buffer is idle
+            if (n.score) cudaFree(n.score);
+            n.score = nullptr;
+            n.score_bytes = 0;
+            if (cudaMalloc(&n.score, bytes) != cudaSuccess) {
+                cudaGetLastError();
+                n.score = nullptr;
+                return fail(DABNN_ERR_OOM, "logprobs: cannot allocate " + std::to_string(bytes) + " bytes");
+            }
+            n.score_bytes = bytes;
+        }
+        unsigned char* d = n.score;
+        if (labels) DABNN_CUDA_OK(cudaMemcpyAsync(d, labels, rows * 8, cudaMemcpyHostToDevice, n.stream));
+        auto f = [&](size_t at) { return reinterpret_cast<float*>(d + at); };
+        auto i = [&](size_t at) { return reinterpret_cast<int64_t*>(d + at); };
+        rc = dabnn_logprobs(logits, DABNN_F32, dims[3], labels ? i(0) : nullptr, (int)rows, dims[3], labels ? f(lp_at) : nullptr, labels ? i(rank_at) : nullptr,
+                            f(entropy_at), top ? f(top_at) : nullptr, top ? i(index_at) : nullptr, top, n.stream);
+        if (rc) return rc;
+        std::vector<unsigned char> host(bytes);
+        const size_t from = labels ? rank_at : index_at;
+        DABNN_CUDA_OK(cudaMemcpyAsync(host.data() + from, d + from, bytes - from, cudaMemcpyDeviceToHost, n.stream));
+        DABNN_CUDA_OK(cudaStreamSynchronize(n.stream));
+        if (labels && label_logprob) memcpy(label_logprob, host.data() + lp_at, rows * 4);
+        if (labels && label_rank) memcpy(label_rank, host.data() + rank_at, rows * 8);
+        if (entropy) memcpy(entropy, host.data() + entropy_at, rows * 4);
+        if (top && top_logprob) memcpy(top_logprob, host.data() + top_at, tops * 4);
+        if (top && top_index) memcpy(top_index, host.data() + index_at, tops * 8);
+    } catch (const std::exception& e) {   // nothing may unwind through the C boundary
+        return fail(DABNN_ERR_OOM, std::string("logprobs: ") + e.what());
+    }
+    return n.check_status();
 }
 extern "C" const char* dabnn_net_output_name(dabnn_net* net, int i) {
     if (!net || i < 0 || i >= (int)net->impl.outputs.size()) return nullptr;

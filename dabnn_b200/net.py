@@ -127,6 +127,25 @@ class Net:
         check(lib.dabnn_net_get_blob_bits(self._h, name.encode(), None, None, out.ctypes.data_as(C.c_void_p), out.size))
         return out
 
+    def logprobs(self, name: str, labels=None, top: int = 0):
+        """Scores a blob of logits of the last run (see dabnn_net_logprobs): (label_logprob, label_rank, entropy, top_logprob,
+        top_index) as numpy arrays [batch, h, w] and [batch, h, w, top], without the unit dimensions h and w of a classifier;
+        None for what was not asked.  labels: int64, one for each row."""
+        shape = self.blob_shape(name)[:3]
+        shape = shape[:1] if shape[1:] == (1, 1) else shape
+        lp = rank = tlp = ti = None
+        if labels is not None:
+            labels = np.ascontiguousarray(labels, dtype=np.int64)
+            if labels.shape != shape:
+                raise ValueError(f"logprobs: expected labels of shape {shape}")
+            lp, rank = np.empty(shape, np.float32), np.empty(shape, np.int64)
+        entropy = np.empty(shape, np.float32)
+        if top:
+            tlp, ti = np.empty((*shape, max(top, 0)), np.float32), np.empty((*shape, max(top, 0)), np.int64)
+        ptr = [None if a is None else a.ctypes.data_as(C.c_void_p) for a in (labels, lp, rank, entropy, tlp, ti)]
+        check(capi.load().dabnn_net_logprobs(self._h, name.encode(), *ptr, top))
+        return lp, rank, entropy, tlp, ti
+
     def get_blob_to_ptr(self, name: str, ptr: int, floats: int):
         check(capi.load().dabnn_net_get_blob(self._h, name.encode(), None, None, C.c_void_p(ptr), floats))
 

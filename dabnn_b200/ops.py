@@ -1,6 +1,7 @@
 """Kernel-level host API over torch CUDA tensors - the Python mirror of the reference's free
 functions (`pack_mat`, `pad`, `im2col`, `fused_binarize_im2col`, `bgemm`, `baseline_bconv` /
-`bconv_3x3`, the float layers), with the same names and argument meaning.
+`bconv_3x3`, the float layers), with the same names and argument meaning - and of what the reference has no
+counterpart for: an 8-bit float product with block scales, and the scoring of logits.
 
 torch is used for device memory and streams only; every function hands raw device pointers to the
 C ABI (include/dabnn_b200.h) and enqueues on torch's current CUDA stream.  Bit tensors are
@@ -302,6 +303,116 @@ def fconv_maxpool(x, weight, bias, pad_h, pad_w, stride_h, stride_w, a=None, b=N
     check(capi.load().dabnn_fconv_maxpool(_ptr(x4), _ptr(_cuda(weight, torch.float32)), _ptr(bias), _ptr(a), _ptr(b), int(relu), _ptr(out),
                                           _ptr(o8), n, h, w, c, cout, kh, kw, pad_h, pad_w, stride_h, stride_w, _stream()))
     return out, o8
+
+
+# ---- 8-bit float matrices with a scale for each block of 128, and the scoring of logits -----------------------------------
+FP8_BLOCK = 128
+_FLOATS = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}   # DABNN_F32 / F16 / BF16
+
+
+def _here(*tensors):
+    """The kernels run on the current device, on its current stream."""
+    device = torch._C._cuda_getDevice()
+    for t in tensors:
+        if t is not None and not (isinstance(t, torch.Tensor) and t.is_cuda and t.device.index == device):
+            raise TypeError("expected CUDA tensors on the current device")
+
+
+def _rows(t, what):
+    """(rows, columns, pitch) of a tensor taken as rows along its last dimension: a matrix with any row pitch, or contiguous."""
+    if t.dim() == 2:
+        rows, cols = t.shape
+        if cols <= 1 or t.stride(1) == 1:
+            return rows, cols, t.stride(0) if rows > 1 else cols
+    elif t.dim() >= 1 and t.is_contiguous():
+        cols = t.shape[-1]
+        return (t.numel() // cols if cols else t.shape[:-1].numel()), cols, cols
+    raise TypeError(f"{what}: expected a matrix with unit stride along its rows, or a contiguous tensor")
+
+
+def _fp8_quantize(x, block_rows):
+    _here(x)
+    kind = _FLOATS.get(x.dtype)
+    if kind is None:
+        raise TypeError("fp8_quantize: expected fp32, fp16 or bf16")
+    rows, k, ld = _rows(x, "fp8_quantize")
+    pitch, blocks = (k + 15) // 16 * 16, (k + FP8_BLOCK - 1) // FP8_BLOCK
+    q = torch.empty((rows, pitch), dtype=torch.float8_e4m3fn, device=x.device)
+    if block_rows == 1:   # block by block: the order in which the product reads them
+        scales = torch.empty((blocks, rows), dtype=torch.float32, device=x.device).t()
+        steps = (1, rows)
+    else:
+        scales = torch.empty(((rows + block_rows - 1) // block_rows, blocks), dtype=torch.float32, device=x.device)
+        steps = (blocks, 1)
+    check(capi.load().dabnn_fp8_quantize(_ptr(x), kind, ld, _ptr(q), pitch, _ptr(scales), *steps, rows, k, block_rows, _stream()))
+    return (q if pitch == k else q[:, :k]), scales
+
+
+def fp8_quantize(x):
+    """Activations [..., K] (fp32, fp16, bf16) -> (e4m3 [..., K], fp32 scales [..., ceil(K / 128)]): one scale, a power of two,
+    for each 128 values of a row (see dabnn_fp8_quantize).  Rows of the result begin on 16-byte boundaries, as fp8_gemm wants
+    them; the scales lie block by block in memory."""
+    q, scales = _fp8_quantize(x, 1)
+    return (q, scales) if x.dim() == 2 else (q.unflatten(0, x.shape[:-1]), scales.unflatten(0, x.shape[:-1])) if x.dim() > 2 else (q[0], scales[0])
+
+
+def fp8_quantize_weights(w):
+    """Weights [N, K] -> (e4m3 [N, K], fp32 scales [ceil(N / 128), ceil(K / 128)]), once per model."""
+    if w.dim() != 2:
+        raise TypeError("fp8_quantize_weights: expected a matrix")
+    return _fp8_quantize(w, FP8_BLOCK)
+
+
+def fp8_gemm(a, a_scales, b, b_scales, bias=None, out_dtype=torch.float32):
+    """[..., K] e4m3 activations times [N, K] e4m3 weights -> [..., N] of out_dtype (fp32, fp16, bf16), + bias (fp32 [N]).
+    Scales as fp8_quantize and fp8_quantize_weights give them, of any value and in any memory order (see dabnn_fp8_gemm)."""
+    _here(a, a_scales, b, b_scales, bias)
+    kind = _FLOATS.get(out_dtype)
+    if kind is None:
+        raise TypeError("fp8_gemm: the result is fp32, fp16 or bf16")
+    if a.dtype != torch.float8_e4m3fn or b.dtype != torch.float8_e4m3fn or a_scales.dtype != torch.float32 or b_scales.dtype != torch.float32:
+        raise TypeError("fp8_gemm: expected float8_e4m3fn operands and fp32 scales")
+    lead = a.shape[:-1]
+    if a.dim() != 2:
+        a = a.unsqueeze(0) if a.dim() == 1 else a.flatten(0, -2)
+        a_scales = a_scales.unsqueeze(0) if a_scales.dim() == 1 else a_scales.flatten(0, -2)
+    if b.dim() != 2:
+        raise TypeError("fp8_gemm: expected a matrix of weights")
+    m, k, lda = _rows(a, "fp8_gemm")
+    n, kb, ldb = _rows(b, "fp8_gemm")
+    blocks = (k + FP8_BLOCK - 1) // FP8_BLOCK
+    if kb != k or a_scales.shape != (m, blocks) or b_scales.shape != ((n + FP8_BLOCK - 1) // FP8_BLOCK, blocks):
+        raise ValueError("fp8_gemm: shapes of the operands and their scales do not go together")
+    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (n,) or not bias.is_contiguous()):
+        raise TypeError("fp8_gemm: expected a contiguous fp32 bias of N values")
+    c = torch.empty((m, n), dtype=out_dtype, device=a.device)
+    check(capi.load().dabnn_fp8_gemm(_ptr(a), lda, _ptr(a_scales), *a_scales.stride(), _ptr(b), ldb, _ptr(b_scales), *b_scales.stride(), _ptr(bias),
+                                     _ptr(c), kind, n, m, n, k, _stream()))
+    return c if len(lead) == 1 else c.unflatten(0, lead) if lead else c[0]
+
+
+def logprobs(logits, labels=None, top=0):
+    """Scores rows of logits [..., classes] (fp32, fp16, bf16) -> (label_logprob, label_rank, entropy, top_logprob, top_index):
+    ln softmax of the class in `labels` (int64 [...]) and how many classes come before it, the entropy, and the `top`
+    likeliest classes with their ln softmax [..., top]; None for what was not asked.  Equal logits rank by index; a
+    negative label is ignored (0 and -1).  Rows with -inf, NaN and other labels: see dabnn_logprobs."""
+    _here(logits, labels)
+    kind = _FLOATS.get(logits.dtype)
+    if kind is None:
+        raise TypeError("logprobs: expected fp32, fp16 or bf16")
+    rows, classes, ld = _rows(logits, "logprobs")
+    lead, device = logits.shape[:-1], logits.device
+    lp = rank = tlp = ti = None
+    if labels is not None:
+        if labels.dtype != torch.int64 or labels.shape != lead or not labels.is_contiguous():
+            raise TypeError("logprobs: expected contiguous int64 labels, one for each row")
+        lp, rank = torch.empty(lead, dtype=torch.float32, device=device), torch.empty(lead, dtype=torch.int64, device=device)
+    entropy = torch.empty(lead, dtype=torch.float32, device=device)
+    if top:
+        tlp, ti = (torch.empty((*lead, max(top, 0)), dtype=t, device=device) for t in (torch.float32, torch.int64))
+    check(capi.load().dabnn_logprobs(_ptr(logits), kind, ld, _ptr(labels), rows, classes, _ptr(lp), _ptr(rank), _ptr(entropy), _ptr(tlp),
+                                     _ptr(ti), top, _stream()))
+    return lp, rank, entropy, tlp, ti
 
 
 def measure_engine_peak(engine):

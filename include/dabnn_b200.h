@@ -52,6 +52,9 @@ enum {
                                 memory; needs N % 16 == 0 and 16-byte aligned rows, otherwise IMMA is used */
 };
 
+/* Element types of the entry points that take more than fp32. */
+enum { DABNN_F32 = 0, DABNN_F16 = 1, DABNN_BF16 = 2 };
+
 typedef void* dabnn_stream_t; /* cudaStream_t */
 
 const char* dabnn_last_error(void);
@@ -218,6 +221,44 @@ int dabnn_fconv_maxpool(const float* in, const float* weight, const float* bias,
                         int pad_w, int stride_h, int stride_w, dabnn_stream_t s);
 
 /* ---------------------------------------------------------------------------------------------
+ * 8-bit float matrices with a scale for each block of 128, and the scoring of logits: a quantised classifier
+ * head.  No counterpart in the reference, whose networks end in a float FC (common/dab.fbs, layers/FloatConv.cpp)
+ * and which does not run Softmax.  Bytes are e4m3 (4 exponent, 3 mantissa bits, largest value 448, 0x7f / 0xff =
+ * NaN).  Pitches and strides are in elements.
+ * ------------------------------------------------------------------------------------------- */
+
+/* in [rows][k] (in_type DABNN_F32 / F16 / BF16, row pitch ld_in) -> out [rows][k] e4m3 (row pitch ld_out), and one
+ * fp32 scale for each block of block_rows x 128 values, block_rows 1 (activations) or 128 (weights); the block of row r
+ * and column c has its scale at scales[r / block_rows * scale_row + c / 128 * scale_block].  Per block, with A the
+ * largest finite magnitude: scale = 2^e, the least e >= -126 with A <= 448 * 2^e, and out = in / scale rounded to nearest
+ * even (the division is exact, so this is the one rounding).  A NaN or an infinity becomes NaN.  Bytes between a row's end
+ * and its pitch are left as they were. */
+int dabnn_fp8_quantize(const void* in, int in_type, long long ld_in, uint8_t* out, long long ld_out, float* scales,
+                       long long scale_row, long long scale_block, int rows, int k, int block_rows, dabnn_stream_t s);
+
+/* c[i][j] = sum over blocks q of 128 along k of as(i, q) * bs(j / 128, q) * sum_{h in q} a[i][h] * b[j][h]  (+ bias[j]),
+ * i < m, j < n: the product of activations [m][k] and weights [n][k], both e4m3, as dabnn_fp8_quantize writes them, with
+ * as(i, q) = a_scales[i * as_row + q * as_block] and bs(j, q) = b_scales[j * bs_row + q * bs_block] of any fp32 value (the
+ * two are multiplied first).  bias fp32 [n] or NULL; c of c_type, row pitch ldc, rounded once from the fp32 sum.  Rows of
+ * a and b begin on 16-byte boundaries (base and pitch), else DABNN_ERR_SHAPE. */
+int dabnn_fp8_gemm(const uint8_t* a, long long lda, const float* a_scales, long long as_row, long long as_block,
+                   const uint8_t* b, long long ldb, const float* b_scales, long long bs_row, long long bs_block,
+                   const float* bias, void* c, int c_type, long long ldc, int m, int n, int k, dabnn_stream_t s);
+
+/* Scores rows of logits [rows][classes] (type DABNN_F32 / F16 / BF16, row pitch ld).  With p = softmax of a row:
+ *   label_logprob[r] = ln p of class labels[r];  label_rank[r] = how many classes come before it (0: the likeliest);
+ *   entropy[r] = -sum p ln p;  top_logprob / top_index [rows][top] = the likeliest classes in order.
+ * Classes are ordered by logit, larger first, equal ones by index.  labels may be NULL (then label_logprob and label_rank
+ * are too) and each output may be NULL, the top pair where top is 0.  top <= DABNN_LOGPROBS_MAX_TOP and <= classes.
+ *  - A class barred with -inf has p = 0 and ln p = -inf.  A row of -inf alone: every ln p is -inf, the entropy 0.
+ *  - A negative label is ignored: logprob 0, rank -1.  A label >= classes: logprob NaN, rank -1.
+ *  - A NaN or +inf in a row: its logprobs and its entropy are NaN; in the order a NaN comes before every number. */
+#define DABNN_LOGPROBS_MAX_TOP 64
+int dabnn_logprobs(const void* logits, int type, long long ld, const int64_t* labels, int rows, int classes,
+                   float* label_logprob, int64_t* label_rank, float* entropy, float* top_logprob, int64_t* top_index,
+                   int top, dabnn_stream_t s);
+
+/* ---------------------------------------------------------------------------------------------
  * Net level: reference dabnn/net.h:22-66 class bnn::Net.
  * ------------------------------------------------------------------------------------------- */
 typedef struct dabnn_net dabnn_net;
@@ -269,6 +310,12 @@ int dabnn_net_wait(dabnn_net* net, int ticket);
  * the layer's output; dims = {batch, h, w, c / 64} words.  Same conventions as dabnn_net_get_blob. */
 int dabnn_net_get_blob_bits(dabnn_net* net, const char* name, int dims[4], const uint64_t** device_ptr,
                             uint64_t* to_host, size_t host_words);
+/* dabnn_logprobs on a blob of the last run (fp32 logits; the rows are its pixels, batch * h * w of them, c the classes) with
+ * host arrays: labels [rows] or NULL, outputs as there, each may be NULL.  Waits for the run and for the results.  Which
+ * blobs can be scored: those dabnn_net_get_blob returns.  The first call allocates a device buffer that later ones of at
+ * most its size use again. */
+int dabnn_net_logprobs(dabnn_net* net, const char* name, const int64_t* labels, float* label_logprob, int64_t* label_rank,
+                       float* entropy, float* top_logprob, int64_t* top_index, int top);
 /* Name of the i-th blob that no layer consumes (network outputs); NULL when i is out of range. */
 const char* dabnn_net_output_name(dabnn_net* net, int i);
 /* The CUDA stream (cudaStream_t) the net enqueues on. */

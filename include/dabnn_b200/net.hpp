@@ -80,6 +80,27 @@ class Net : public std::enable_shared_from_this<Net> {
         check(dabnn_net_get_blob_bits(handle_, name.c_str(), nullptr, nullptr, words.data(), words.size()));
         return words;
     }
+    // Scores of a blob of logits of the last run, one row per pixel (for a classifier: per image); no counterpart in the
+    // reference.  labels: one class per row, or null; top: how many alternatives of each row, [rows][top].
+    struct Scores {
+        std::vector<float> label_logprob, entropy, top_logprob;
+        std::vector<int64_t> label_rank, top_index;
+    };
+    Scores logprobs(const std::string& name, const int64_t* labels = nullptr, int top = 0) {
+        int dims[4];
+        const int rc = dabnn_net_get_blob(handle_, name.c_str(), dims, nullptr, nullptr, 0);
+        if (rc == DABNN_ERR_NOT_FOUND) throw std::out_of_range(dabnn_last_error());
+        check(rc);
+        const size_t rows = static_cast<size_t>(dims[0]) * dims[1] * dims[2], tops = rows * static_cast<size_t>(top > 0 ? top : 0);
+        Scores s;
+        s.entropy.resize(rows);
+        if (labels) { s.label_logprob.resize(rows); s.label_rank.resize(rows); }
+        s.top_logprob.resize(tops);
+        s.top_index.resize(tops);
+        check(dabnn_net_logprobs(handle_, name.c_str(), labels, labels ? s.label_logprob.data() : nullptr, labels ? s.label_rank.data() : nullptr,
+                                 s.entropy.data(), s.top_logprob.data(), s.top_index.data(), top));
+        return s;
+    }
     dabnn_net* handle() const { return handle_; }
 
    private:

@@ -1,0 +1,304 @@
+"""8-bit float matrices with a scale for each block of 128: quantiser and product against their 64-bit forms."""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+import head_reference as R  # noqa: E402
+
+TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from dabnn_b200 import ops as o
+    yield o
+    assert o.engine_status() == 0
+
+
+def values(t):
+    return t.float().cpu().double().numpy()
+
+
+def same(got, expected):
+    np.testing.assert_array_equal(values(got), expected)
+
+
+# ---------------------------------------------------------------------------------------------- quantiser
+def check_quantize(ops, x, weights):
+    q, s = ops.fp8_quantize_weights(x) if weights else ops.fp8_quantize(x)
+    eq, es = R.quantize(values(x), 128 if weights else 1)
+    assert q.dtype == torch.float8_e4m3fn and s.dtype == torch.float32 and q.shape == x.shape
+    same(s, es)
+    same(q, eq)
+    assert x.shape[0] <= 1 or q.stride(0) % 16 == 0
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("weights", [False, True])
+@pytest.mark.parametrize("rows,k", [(1, 1), (1, 4096), (3, 127), (5, 128), (130, 129), (64, 257), (129, 1000), (257, 512)])
+def test_quantize(ops, rows, k, weights, kind):
+    g = torch.Generator().manual_seed(rows * 7 + k)
+    x = torch.randn((rows, k), generator=g) * torch.exp(3 * torch.randn((rows, 1), generator=g))
+    check_quantize(ops, x.to(TYPES[kind]).cuda(), weights)
+
+
+@pytest.mark.parametrize("weights", [False, True])
+def test_quantize_borders(ops, weights):
+    """Magnitudes at and next to 448 2^e, ties between e4m3 values, subnormal bytes, zero blocks, the ends of fp32."""
+    x = torch.zeros((10, 640))
+    x[0, :4] = torch.tensor([448.0, -447.99997, 1.0, 0.0])
+    x[1, :3] = torch.tensor([448.00003, -1.0, 0.3])
+    x[2, :6] = torch.tensor([256.0, 17.0, 19.0, -17.0, 21.0, 18.999998])             # ties between 16, 18, 20
+    x[3, :6] = torch.tensor([300.0, 2.0 ** -9, 2.0 ** -10, 3 * 2.0 ** -10, -(2.0 ** -11), 1e-5])
+    x[4, 128:132] = torch.tensor([3.4028235e38, -1.0, 1e30, 2.0 ** 118])
+    x[5, 256:260] = torch.tensor([1.1754944e-38, 1e-45, -1e-45, 5e-39])
+    x[6, 384:387] = torch.tensor([2.0 ** -117, -(2.0 ** -126), 2.0 ** -135])
+    x[7, 639] = -1.75
+    x[8, 500] = 1.7500001
+    x[9, :640] = torch.arange(640) * 0.7 - 224
+    check_quantize(ops, x.cuda(), weights)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("weights", [False, True])
+def test_quantize_not_finite(ops, weights, kind):
+    """NaN and infinities become NaN; the scale and the other values of their block are those without them."""
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn((140, 300), generator=g)
+    for v, at in ((float("nan"), (3, 5)), (float("inf"), (3, 6)), (-float("inf"), (7, 299)), (float("nan"), (139, 128))):
+        x[at] = v
+    x[9, 128:256] = float("inf")      # nothing finite in the block
+    check_quantize(ops, x.to(TYPES[kind]).cuda(), weights)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_quantize_strided_rows_and_offsets(ops, kind):
+    """Rows with a pitch, bases off every vector boundary, leading dimensions."""
+    g = torch.Generator().manual_seed(4)
+    store = torch.randn((33, 1003), generator=g).to(TYPES[kind]).cuda()
+    for first in (0, 1, 3, 8):
+        for k in (130, 512, 900):
+            x = store[:, first:first + k]
+            for weights in (False, True):
+                check_quantize(ops, x, weights)
+    x = store[:24, :600].contiguous().view(2, 3, 4, 600)
+    q, s = ops.fp8_quantize(x)
+    assert q.shape == (2, 3, 4, 600) and s.shape == (2, 3, 4, 5)
+    eq, es = R.quantize(values(x.view(24, 600)), 1)
+    same(q.reshape(24, 600), eq)
+    same(s.reshape(24, 5), es)
+    q1, s1 = ops.fp8_quantize(store[2, :600])
+    same(q1, eq[2])
+    same(s1, es[2])
+
+
+def test_quantize_leaves_the_rest_alone(ops):
+    """Bytes behind a row's end, rows and scales behind the last: as they were; any strides of the scales."""
+    from dabnn_b200 import capi
+    x = torch.randn((5, 200), device="cuda")
+    out = torch.full((8, 256), 0x55, dtype=torch.uint8, device="cuda")
+    scales = torch.full((8, 9), -7.0, device="cuda")
+    capi.check(capi.load().dabnn_fp8_quantize(x.data_ptr(), 0, 200, out.data_ptr(), 256, scales.data_ptr(), 9, 4, 5, 200, 1, ops._stream()))
+    eq, es = R.quantize(values(x), 1)
+    same(out[:5, :200].view(torch.float8_e4m3fn), eq)
+    same(scales[:5, 0:5:4], es)
+    assert (out[5:] == 0x55).all() and (out[:, 200:] == 0x55).all()
+    scales[:5, 0:5:4] = -7
+    assert (scales == -7).all()
+
+
+def test_quantize_empty(ops):
+    for shape in ((0, 256), (4, 0), (0, 0)):
+        q, s = ops.fp8_quantize(torch.empty(shape, device="cuda"))
+        assert q.shape == shape and s.shape == (shape[0], -(-shape[1] // 128))
+
+
+# ---------------------------------------------------------------------------------------------- product
+def operands(m, n, k, seed, powers=False):
+    """Values of e4m3 bytes (every finite one occurs) and scales of either sign, as 64-bit arrays."""
+    rng = np.random.default_rng(seed)
+    table = torch.arange(256, dtype=torch.uint8).view(torch.float8_e4m3fn).double().numpy()
+    table = table[np.isfinite(table)]
+    a, b = rng.choice(table, (m, k)), rng.choice(table, (n, k))
+    nk = -(-k // 128)
+
+    def scales(rows):
+        s = np.exp2(rng.integers(-6, 6, (rows, nk)).astype(np.float64))
+        return s if powers else (s * rng.uniform(-1.5, 1.5, (rows, nk))).astype(np.float32).astype(np.float64)
+
+    return a, scales(m), b, scales(-(-n // 128)), rng.normal(0, 100, n).astype(np.float32).astype(np.float64)
+
+
+def dev(a):
+    return torch.from_numpy(a).float().cuda()
+
+
+def check_gemm(ops, m, n, k, out="f32", bias=True, seed=None):
+    a, sa, b, sb, bv = operands(m, n, k, seed if seed is not None else m * 31 + n * 7 + k)
+    if not bias:
+        bv = None
+    dt = TYPES[out]
+    if out == "f16":                                                # keep the results inside the type
+        sa, sb = sa * 2.0 ** -14, sb * 2.0 ** -6
+    c, tol = R.gemm(a, sa, b, sb, bv, torch.finfo(dt).eps)
+    got = ops.fp8_gemm(R.f8(a), dev(sa), R.f8(b), dev(sb), None if bv is None else dev(bv), dt)
+    assert got.dtype == dt
+    # fp16 results below its normal range step by 2^-24
+    R.close(values(got), c, tol + (2.0 ** -25 if out == "f16" else 0.0))
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 8, 16), (1, 128, 128), (2, 129, 144), (3, 1000, 512), (5, 17, 257), (8, 4100, 1300), (15, 257, 640),
+                                   (16, 512, 2048), (17, 130, 129), (31, 640, 384), (33, 64, 4096), (37, 4100, 2064), (63, 1, 300), (64, 129, 1000)])
+def test_gemm_few_rows(ops, m, n, k):
+    check_gemm(ops, m, n, k)
+
+
+@pytest.mark.parametrize("m,n,k", [(65, 128, 128), (100, 1000, 512), (127, 255, 257), (128, 128, 256), (129, 1, 128), (200, 2050, 96), (255, 300, 130),
+                                   (256, 256, 1024), (257, 513, 1025), (1024, 1000, 512), (700, 1300, 64)])
+def test_gemm_many_rows(ops, m, n, k):
+    check_gemm(ops, m, n, k)
+
+
+def test_gemm_large(ops):
+    """More tiles than SMs in both directions, long K."""
+    check_gemm(ops, 2300, 4200, 700)
+    check_gemm(ops, 300, 520, 16400)
+
+
+@pytest.mark.parametrize("out", TYPES)
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("m,n,k", [(1, 1000, 512), (20, 131, 300), (150, 259, 384), (300, 1001, 200)])
+def test_gemm_output_types(ops, m, n, k, out, bias):
+    check_gemm(ops, m, n, k, out, bias)
+
+
+def test_gemm_without_k_and_empty(ops):
+    bias = torch.randn(9, device="cuda")
+    a, b = torch.empty((4, 0), device="cuda").to(torch.float8_e4m3fn), torch.empty((9, 0), device="cuda").to(torch.float8_e4m3fn)
+    e = torch.empty((4, 0), device="cuda")
+    assert torch.equal(ops.fp8_gemm(a, e, b, torch.empty((1, 0), device="cuda"), bias), bias.expand(4, 9))
+    assert torch.equal(ops.fp8_gemm(a, e, b, torch.empty((1, 0), device="cuda")), torch.zeros((4, 9), device="cuda"))
+    a, s = ops.fp8_quantize(torch.randn((0, 256), device="cuda"))
+    b, t = ops.fp8_quantize_weights(torch.randn((130, 256), device="cuda"))
+    assert ops.fp8_gemm(a, s, b, t).shape == (0, 130)
+    assert ops.fp8_gemm(b, t.repeat_interleave(128, 0)[:130], a, torch.empty((0, 2), device="cuda")).shape == (130, 0)
+
+
+@pytest.mark.parametrize("m", [3, 40, 200])
+def test_gemm_strides(ops, m):
+    """Operands with row pitches, scales in either memory order, inside larger tensors, an output with a pitch."""
+    from dabnn_b200 import capi
+    n, k = 200, 272
+    a, sa, b, sb, bias = operands(m, n, k, 5)
+    c, tol = R.gemm(a, sa, b, sb, bias, torch.finfo(torch.float32).eps)
+    wide_a, wide_b = torch.zeros((m, 336), dtype=torch.float8_e4m3fn, device="cuda"), torch.zeros((n, 400), dtype=torch.float8_e4m3fn, device="cuda")
+    wide_a.view(torch.uint8).fill_(0x7f)   # NaN around the operands
+    wide_b.view(torch.uint8).fill_(0x7f)
+    wide_a[:, 16:16 + k] = R.f8(a)
+    wide_b[:, 32:32 + k] = R.f8(b)
+    va, vb = wide_a[:, 16:16 + k], wide_b[:, 32:32 + k]
+    store = torch.full((m, 7), float("nan"), device="cuda")
+    store[:, 1:7:2] = dev(sa)
+    for s in (dev(sa), dev(sa).t().contiguous().t(), store[:, 1:7:2]):
+        for t in (dev(sb), dev(sb).t().contiguous().t()):
+            R.close(values(ops.fp8_gemm(va, s, vb, t, dev(bias))), c, tol)
+    out = torch.full((m + 2, n + 13), -5.0, device="cuda")
+    s, t = dev(sa), dev(sb)
+    capi.check(capi.load().dabnn_fp8_gemm(va.data_ptr(), 336, s.data_ptr(), *s.stride(), vb.data_ptr(), 400, t.data_ptr(), *t.stride(), dev(bias).data_ptr(),
+                                          out.data_ptr() + 4 * 5, 0, n + 13, m, n, k, ops._stream()))
+    R.close(values(out[:m, 5:5 + n]), c, tol)
+    out[:m, 5:5 + n] = -5
+    assert (out == -5).all()
+
+
+@pytest.mark.parametrize("m,n", [(4, 300), (90, 300), (300, 300)])
+def test_gemm_special_values(ops, m, n):
+    """NaN bytes reach the outputs of their row and column and no other; scales of zero; blocks of zeros."""
+    k = 400
+    a, sa, b, sb, _ = operands(m, n, k, 6, powers=True)
+    a[m // 2, 130:250] = 0
+    c, tol = R.gemm(a, sa, b, sb, None, torch.finfo(torch.float32).eps)
+    qa, qb = R.f8(a), R.f8(b)
+    qa[1, 399] = float("nan")
+    qb[257, 3] = float("nan")
+    got = values(ops.fp8_gemm(qa, dev(sa), qb, dev(sb)))
+    expected = c.copy()
+    expected[1, :] = np.nan
+    expected[:, 257] = np.nan
+    R.close(got, expected, tol)
+    sz = sa.copy()
+    sz[2, :] = 0
+    got = values(ops.fp8_gemm(R.f8(a), dev(sz), R.f8(b), dev(sb)))
+    assert (got[2] == 0).all()
+
+
+@pytest.mark.parametrize("m,n,k", [(2, 1000, 4096), (40, 520, 2048), (300, 700, 512)])
+def test_gemm_is_deterministic_and_row_independent(ops, m, n, k):
+    """The same bits each time; a row's results do not depend on what the other rows hold."""
+    a, sa, b, sb, bias = operands(m, n, k, 8)
+    args = (R.f8(b), dev(sb), dev(bias))
+    first = ops.fp8_gemm(R.f8(a), dev(sa), *args)
+    for _ in range(3):
+        assert torch.equal(ops.fp8_gemm(R.f8(a), dev(sa), *args), first)
+    other, so, _, _, _ = operands(m, n, k, 9)
+    other[1], so[1] = a[1], sa[1]
+    assert torch.equal(ops.fp8_gemm(R.f8(other), dev(so), *args)[1], first[1])
+
+
+def test_gemm_leading_dimensions_streams_and_graphs(ops):
+    """[2, 3, K] activations; a side stream; capture and replay with new contents, two graphs in turn."""
+    g = torch.Generator().manual_seed(1)
+    x, w = torch.randn((2, 3, 320), generator=g).cuda(), torch.randn((150, 320), generator=g).cuda()
+    q, s = ops.fp8_quantize(x)
+    b, t = ops.fp8_quantize_weights(w)
+    plain = ops.fp8_gemm(q, s, b, t)
+    assert plain.shape == (2, 3, 150)
+    assert torch.equal(ops.fp8_gemm(q[1, 2], s[1, 2], b, t), plain[1, 2])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = ops.fp8_gemm(q, s, b, t)
+    side.synchronize()
+    assert torch.equal(other, plain)
+    graphs = []
+    xs = [x.clone(), x.clone()]
+    for xi in xs:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            qi, si = ops.fp8_quantize(xi)
+            ci = ops.fp8_gemm(qi, si, b, t)
+        graphs.append((graph, ci))
+    for i in (0, 1, 0):
+        xs[i].mul_(-2.0)
+        expected = ops.fp8_gemm(*ops.fp8_quantize(xs[i]), b, t)
+        graphs[i][0].replay()
+        assert torch.equal(graphs[i][1], expected)
+
+
+# ---------------------------------------------------------------------------------------------- the head as a whole
+@pytest.mark.parametrize("m,classes,k", [(1, 1000, 512), (64, 1000, 512), (200, 365, 1100)])
+def test_classifier_head(ops, m, classes, k):
+    """Features -> bytes -> logits -> scores, each step against the 64-bit form of what went into it."""
+    g = torch.Generator().manual_seed(m + classes)
+    x, w, bias = torch.randn((m, k), generator=g).cuda(), (torch.randn((classes, k), generator=g) * 4 * k ** -0.5).cuda(), torch.randn(classes, generator=g).cuda()
+    labels = torch.randint(0, classes, (m,), generator=g).cuda()
+    wq, ws = ops.fp8_quantize_weights(w)
+    q, s = ops.fp8_quantize(x)
+    logits = ops.fp8_gemm(q, s, wq, ws, bias)
+    lp, rank, entropy, tlp, ti = ops.logprobs(logits, labels, 5)
+    c, tol = R.gemm(*R.quantize(values(x), 1), *R.quantize(values(w), 128), values(bias), torch.finfo(torch.float32).eps)
+    R.close(values(logits), c, tol)
+    expected, tols = R.logprobs(values(logits), labels.cpu().numpy(), 5)
+    for got, e, t in zip((lp, entropy, tlp), (expected[0], expected[2], expected[3]), tols):
+        R.close(got.cpu(), e, t)
+    np.testing.assert_array_equal(rank.cpu(), expected[1])
+    np.testing.assert_array_equal(ti.cpu(), expected[4])
+    # the bytes cost little: rounding is off by at most 2^-4 of a value or half of 2^-9 of the block's scale
+    exact = values(x) @ values(w).T + values(bias)
+    ax, aw = np.abs(values(x)), np.abs(values(w))
+    sx = np.repeat(R.quantize(values(x), 1)[1], 128, 1)[:, :k] * 2.0 ** -10
+    sw = np.repeat(np.repeat(R.quantize(values(w), 128)[1], 128, 0)[:classes], 128, 1)[:, :k] * 2.0 ** -10
+    ex, ew = np.maximum(ax * 2.0 ** -4, sx), np.maximum(aw * 2.0 ** -4, sw)
+    R.close(values(logits), exact, tol + ex @ aw.T + ax @ ew.T + ex @ ew.T)

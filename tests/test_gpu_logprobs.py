@@ -1,0 +1,221 @@
+"""Scoring of logits against its 64-bit form: kernel level and on a Net's output."""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+import head_reference as R  # noqa: E402
+
+TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+INF, NAN = float("inf"), float("nan")
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from dabnn_b200 import ops as o
+    return o
+
+
+def check(ops, logits, labels, top):
+    """logits on the device, labels a list or None"""
+    lab = None if labels is None else torch.tensor(labels, dtype=torch.int64)
+    got = ops.logprobs(logits, None if lab is None else lab.cuda(), top)
+    (lp, rank, ent, tlp, ti), (tol, etol, ttol) = R.logprobs(logits.float().cpu().numpy(), None if lab is None else lab.numpy(), top)
+    if labels is None:
+        assert got[0] is None and got[1] is None
+    else:
+        np.testing.assert_array_equal(got[1].cpu(), rank)
+        R.close(got[0].cpu(), lp, tol)
+    R.close(got[2].cpu(), ent, etol)
+    if top:
+        np.testing.assert_array_equal(got[4].cpu(), ti)
+        R.close(got[3].cpu(), tlp, ttol)
+    else:
+        assert got[3] is None and got[4] is None
+
+
+def rows_of(rows, classes, seed, kind, spread=3.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn((rows, classes), generator=g) * spread).to(TYPES[kind]).cuda(), torch.randint(0, classes, (rows,), generator=g).tolist()
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("classes", [1, 2, 7, 31, 32, 33, 100, 255, 1000, 1023, 1024, 1025, 2048, 4097, 8191, 8192, 8193])
+def test_logprobs(ops, classes, kind):
+    for rows in (1, 3, 40):
+        x, labels = rows_of(rows, classes, classes + rows, kind)
+        for top in sorted({0, 1, min(5, classes), min(20, classes), min(64, classes)}):
+            check(ops, x, labels, top)
+    check(ops, x, None, min(3, classes))
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("rows,classes,top", [(1, 131072, 20), (2, 50000, 5), (3, 262144, 64), (1, 65537, 32), (150, 20001, 8), (400, 12345, 5)])
+def test_logprobs_wide(ops, rows, classes, top, kind):
+    x, labels = rows_of(rows, classes, classes + rows, kind)
+    check(ops, x, labels, top)
+
+
+def test_logprobs_many_rows(ops):
+    x, labels = rows_of(5000, 10, 1, "f32")
+    check(ops, x, labels, 3)
+    x, labels = rows_of(1024, 1000, 2, "f32")
+    check(ops, x, labels, 5)
+
+
+@pytest.mark.parametrize("classes", [70, 1000, 9000, 40000])
+@pytest.mark.parametrize("kind", TYPES)
+def test_ties_and_orders(ops, classes, kind):
+    """Constant rows, few distinct values, both zeros, rising and falling rows, everything large at the end."""
+    x = torch.zeros((8, classes))
+    x[1] = 3.0
+    x[2] = torch.arange(classes) % 3
+    x[3, 1::2] = -0.0
+    x[4] = torch.arange(classes) / classes * 8
+    x[5] = -torch.arange(classes) / classes * 8
+    x[6, -5:] = 7.0
+    x[7] = (torch.arange(classes) * 7919 % 101).float()
+    for label in (0, classes // 2, classes - 1):
+        check(ops, x.to(TYPES[kind]).cuda(), [label] * 8, 5)
+    check(ops, x.to(TYPES[kind]).cuda(), [classes - 3] * 8, 64)
+
+
+@pytest.mark.parametrize("classes", [70, 1000, 9000, 140000])
+@pytest.mark.parametrize("kind", TYPES)
+def test_barred_classes_and_special_values(ops, classes, kind):
+    """-inf, the type's lowest value, +inf and NaN: rows with few classes left, one, none."""
+    lowest = torch.finfo(TYPES[kind]).min
+    g = torch.Generator().manual_seed(classes)
+    x = (torch.randn((14, classes), generator=g) * 3).to(TYPES[kind])
+    x[0] = -INF
+    x[1] = -INF
+    x[1, classes - 2] = 1.5
+    x[2, 3:] = -INF
+    x[3, ::2] = -INF
+    x[4] = lowest
+    x[5, 2:] = lowest
+    x[6, classes // 3] = NAN
+    x[7, classes // 3] = INF
+    x[8] = NAN
+    x[9] = -INF
+    x[9, 5] = NAN
+    x[10, 5], x[10, 6] = INF, -INF
+    x[11] = torch.finfo(TYPES[kind]).max
+    x[12, 1:] = lowest
+    x[12, 0] = torch.finfo(TYPES[kind]).max
+    x[13, 0::2], x[13, 1::2] = -NAN, NAN
+    labels = [0, classes - 2, 1, 2, classes - 1, 7, 3, classes // 3, 4, 5, 6, 9, 1, 2]
+    check(ops, x.cuda(), labels, 8)
+    check(ops, x.cuda(), labels, 0)
+
+
+@pytest.mark.parametrize("classes", [5, 1000, 20000])
+def test_labels_outside(ops, classes):
+    x, _ = rows_of(6, classes, 3, "f32")
+    check(ops, x, [-1, -100, classes, classes + 7, 2**62, -2**63], 2)
+    check(ops, x, [0, classes - 1, -1, classes, 1, 2], 0)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("classes", [100, 1000, 9001])
+def test_strided_rows_and_offsets(ops, kind, classes):
+    """Row pitches and bases off every vector boundary; what lies around the rows is not read into them."""
+    store = torch.full((9, classes + 37), NAN, dtype=TYPES[kind]).cuda()
+    for first in (0, 1, 2, 4, 8, 13):
+        x = store[:, first:first + classes]
+        x.copy_(rows_of(9, classes, first, kind)[0])
+        check(ops, x, list(range(9)), 6)
+        x.fill_(NAN)
+
+
+def test_shapes(ops):
+    x, labels = rows_of(24, 50, 1, "bf16")
+    lab = torch.tensor(labels).cuda()
+    flat = ops.logprobs(x, lab, 4)
+    deep = ops.logprobs(x.view(2, 3, 4, 50), lab.view(2, 3, 4), 4)
+    for f, d in zip(flat, deep):
+        assert d.shape[:3] == (2, 3, 4) and torch.equal(f, d.reshape(f.shape))
+    one = ops.logprobs(x[5], lab[5], 4)
+    for f, d in zip(flat, one):
+        assert torch.equal(f[5], d)
+    for t in ops.logprobs(torch.empty((0, 50), device="cuda"), torch.empty(0, dtype=torch.int64, device="cuda"), 4):
+        assert t.shape[0] == 0
+
+
+@pytest.mark.parametrize("rows,classes", [(2, 1000), (3, 30000)])
+def test_same_bits_alone_and_in_a_batch(ops, rows, classes):
+    x, labels = rows_of(rows, classes, 7, "f32")
+    lab = torch.tensor(labels).cuda()
+    first = ops.logprobs(x, lab, 5)
+    for _ in range(3):
+        for a, b in zip(first, ops.logprobs(x, lab, 5)):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("rows,classes", [(3, 1000), (2, 40000)])
+def test_streams_and_graphs(ops, rows, classes):
+    x, labels = rows_of(rows, classes, 9, "f32")
+    lab = torch.tensor(labels).cuda()
+    plain = ops.logprobs(x, lab, 5)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = ops.logprobs(x, lab, 5)
+    side.synchronize()
+    for a, b in zip(plain, other):
+        assert torch.equal(a, b)
+    xs, graphs = [x.clone(), x.clone()], []
+    for xi in xs:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = ops.logprobs(xi, lab, 5)
+        graphs.append((graph, out))
+    for i in (0, 1, 0):
+        xs[i].mul_(-0.5)
+        graphs[i][0].replay()
+        for a, b in zip(graphs[i][1], ops.logprobs(xs[i], lab, 5)):
+            assert torch.equal(a, b)
+
+
+def test_offsets_beyond_32_bits(ops):
+    """Rows that begin beyond 2^32 elements of the base."""
+    classes, pitch = 1000, 1 << 31
+    store = torch.zeros((2 * pitch + classes) // 2 * 2, dtype=torch.bfloat16, device="cuda")
+    x = store.as_strided((3, classes), (pitch, 1))
+    x.copy_(rows_of(3, classes, 11, "bf16")[0])
+    check(ops, x, [1, 2, 3], 5)
+
+
+def test_net_logprobs(ops):
+    """The scores of a Net's own logits: as the kernel-level call gives them, in either plan, batches of several sizes."""
+    from dabnn_b200.bireal import OUTPUT_BLOB, build_bireal18
+    from dabnn_b200.capi import DabnnError
+    from dabnn_b200.dab_format import write_dab
+    from dabnn_b200.net import Net
+    rng = np.random.default_rng(0)
+    model = write_dab(build_bireal18(image_hw=64, num_classes=100))
+    for optimize in (True, False):
+        net = Net.create()
+        net.max_batch, net.optimize = 5, optimize
+        net.read_buf(model)
+        with pytest.raises(DabnnError):
+            net.logprobs(OUTPUT_BLOB)                       # nothing has been run
+        for batch in (2, 5, 1):
+            net.run(rng.normal(0, 1, (batch, 64, 64, 3)).astype(np.float32))
+            logits = net.get_blob(OUTPUT_BLOB).reshape(batch, 100)
+            labels = rng.integers(0, 100, batch)
+            lp, rank, ent, tlp, ti = net.logprobs(OUTPUT_BLOB, labels, top=5)
+            for got, e in zip((lp, rank, ent, tlp, ti), ops.logprobs(torch.from_numpy(logits).cuda(), torch.from_numpy(labels).cuda(), 5)):
+                np.testing.assert_array_equal(got, e.cpu().numpy())
+            assert (ti[:, 0] == logits.argmax(1)).all()
+            only = net.logprobs(OUTPUT_BLOB)
+            assert only[0] is None and only[4] is None
+            np.testing.assert_array_equal(only[2], ent)
+        with pytest.raises(DabnnError):
+            net.logprobs(OUTPUT_BLOB, top=65)
+        with pytest.raises(KeyError):
+            net.logprobs("no such blob")
+        with pytest.raises(ValueError):
+            net.logprobs(OUTPUT_BLOB, labels=[1, 2, 3])
+        net.close()
