@@ -341,9 +341,9 @@ int dabnn::contraction_status_word(int** addr) {
 extern "C" int dabnn_last_engine(void) { return g_last_engine; }
 
 extern "C" int dabnn_debug_raise_engine_status(int which, int code) {
-    DABNN_REQUIRE(which >= 0 && which <= 2, DABNN_ERR_ARG, "raise_engine_status: which must be 0, 1 or 2");
+    DABNN_REQUIRE(which >= 0 && which <= 3, DABNN_ERR_ARG, "raise_engine_status: which must be 0, 1, 2 or 3");
     int* word = nullptr;
-    const int rc = which == 0 ? contraction_status_word(&word) : which == 1 ? fconv_status_word(&word) : bconv_u8_status_word(&word);
+    const int rc = which == 0 ? contraction_status_word(&word) : which == 1 ? fconv_status_word(&word) : which == 2 ? bconv_u8_status_word(&word) : fp8_status_word(&word);
     if (rc) return rc;
     DABNN_CUDA_OK(cudaMemcpy(word, &code, sizeof(int), cudaMemcpyHostToDevice));
     return DABNN_OK;
@@ -357,6 +357,15 @@ extern "C" int dabnn_engine_status(int* status) {
         const int rc = fconv_tc5_status(status);
         if (rc) return rc;
     }
-    if (*status == 0) return bconv_u8_status(status);
+    if (*status == 0) {
+        const int rc = bconv_u8_status(status);
+        if (rc) return rc;
+    }
+    if (*status == 0) {   // the 8-bit float product (51-54)
+        int* word = nullptr;
+        const int rc = fp8_status_word(&word);
+        if (rc) return rc;
+        DABNN_CUDA_OK(cudaMemcpy(status, word, sizeof(int), cudaMemcpyDeviceToHost));
+    }
     return DABNN_OK;
 }

@@ -1,17 +1,13 @@
 // 8-bit float matrices with a scale for each block of 128: the quantiser and the product.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
 #include <algorithm>
+#include <climits>
 
-#include "common.cuh"
+#include "fp8_gemm.cuh"
 #include "kernels.h"
-#include "scalar_types.cuh"
 
 namespace dabnn {
-
-constexpr int F8_BLOCK = 128;
 
 // The scale of a block whose largest finite magnitude has the bits `top` (fp32): the least power of two 2^e, e >= -126, with
 // top <= 448 * 2^e, 448 = 1.75 * 2^8 being the largest e4m3 value.  As bits; the reciprocal's bits are (254 << 23) - scale.
@@ -48,31 +44,85 @@ __global__ void __launch_bounds__(128) fp8_quantize_kernel(const T* __restrict__
     }
 }
 
-__device__ __forceinline__ float f8_to_f32(uint8_t v) { return __half2float(__half(__nv_cvt_fp8_to_halfraw(v, __NV_E4M3))); }
+// -------------------------------------------------------------------------------------------------
+// The product: which tile, how many CTAs share one.
+static int f8_tokens_of_tile(int m, int n) {
+    if (m <= 16) return 16;
+    if (m <= 32) return 32;
+    const long long tiles_n = (n + 127) / 128;
+    if (m <= 64 || tiles_n * ((m + 127) / 128) < sm_count()) return 64;
+    return tiles_n * ((m + 255) / 256) < sm_count() ? 128 : 256;
+}
+static int f8_splits(long long ntiles, int nkb) {
+    int s = 1;
+    while (s < F8_MAX_SPLIT && 2 * s * ntiles <= 2 * sm_count() && 4 * s <= nkb) s *= 2;
+    return s;
+}
 
-// 16 x 16 outputs per CTA, one block of K at a time
-template <typename T>
-__global__ void __launch_bounds__(256) fp8_gemm_kernel(const uint8_t* __restrict__ a, const long long lda, const float* __restrict__ as, const long long as_row,
-                                                       const long long as_block, const uint8_t* __restrict__ b, const long long ldb,
-                                                       const float* __restrict__ bs, const long long bs_row, const long long bs_block,
-                                                       const float* __restrict__ bias, T* __restrict__ c, const long long ldc, const int M, const int N, const int K) {
-    __shared__ float sa[16][F8_BLOCK + 1], sb[16][F8_BLOCK + 1];
-    const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
-    const long long m0 = (long long)blockIdx.y * 16, n0 = (long long)blockIdx.x * 16;
-    float acc = 0.f;
-    for (int kb = 0; kb * F8_BLOCK < K; kb++) {
-        for (int i = threadIdx.x; i < 16 * F8_BLOCK; i += 256) {
-            const int r = i >> 7, k = kb * F8_BLOCK + (i & 127);
-            sa[r][i & 127] = k < K && m0 + r < M ? f8_to_f32(a[(m0 + r) * lda + k]) : 0.f;
-            sb[r][i & 127] = k < K && n0 + r < N ? f8_to_f32(b[(n0 + r) * ldb + k]) : 0.f;
-        }
-        __syncthreads();
-        float part = 0.f;
-        for (int k = 0; k < F8_BLOCK; k++) part = fmaf(sa[ty][k], sb[tx][k], part);
-        if (m0 + ty < M && n0 + tx < N) acc = fmaf(as[(m0 + ty) * as_row + kb * as_block] * bs[((n0 + tx) >> 7) * bs_row + kb * bs_block], part, acc);
-        __syncthreads();
+template <int NT, bool SPLIT, typename T>
+static int f8_launch(const Fp8Params& p, int splits, const CUtensorMap& w_map, const CUtensorMap& x_map, cudaStream_t stream) {
+    using Cfg = Fp8Cfg<NT>;
+    auto kern = fp8_gemm_kernel<NT, SPLIT, T>;
+    static thread_local int ready_device = -1;
+    int dev = 0;
+    DABNN_CUDA_OK(cudaGetDevice(&dev));
+    if (dev != ready_device) {
+        DABNN_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM));
+        ready_device = dev;
     }
-    if (m0 + ty < M && n0 + tx < N) c[(m0 + ty) * ldc + n0 + tx] = from_f32<T>(acc + (bias ? bias[n0 + tx] : 0.f));
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(SPLIT ? p.ntiles * splits : std::min(p.ntiles, sm_count() * Cfg::CTAS_PER_SM));
+    cfg.blockDim = dim3(Cfg::THREADS);
+    cfg.dynamicSmemBytes = Cfg::SMEM;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    int n = 0;
+    if (g_overlap_launches) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (SPLIT) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = splits;
+        attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+        n++;
+    }
+    cfg.attrs = attr;
+    cfg.numAttrs = n;
+    DABNN_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, p, splits, w_map, x_map));
+    return DABNN_OK;
+}
+
+template <typename T>
+static int f8_gemm(Fp8Params p, const uint8_t* a, long long lda, const uint8_t* b, long long ldb, int k, cudaStream_t stream) {
+    const int nt = f8_tokens_of_tile(p.M, p.N);
+    p.tiles_n = (p.N + 127) / 128;
+    const long long ntiles = (long long)p.tiles_n * ((p.M + nt - 1) / nt);
+    DABNN_REQUIRE(ntiles < (1ll << 30), DABNN_ERR_SHAPE, "fp8_gemm: too many outputs");
+    p.ntiles = (int)ntiles;
+    p.nkb = (k + F8_BLOCK - 1) / F8_BLOCK;
+    CUtensorMap w_map{}, x_map{};
+    if (k > 0) {   // a single row's pitch is of no account, but the descriptor wants one
+        const unsigned long long whole = ((unsigned long long)k + 15) / 16 * 16;
+        const unsigned long long wdims[2] = {(unsigned long long)k, (unsigned long long)p.N}, wpitch[1] = {p.N > 1 ? (unsigned long long)ldb : whole};
+        const unsigned long long xdims[2] = {(unsigned long long)k, (unsigned long long)p.M}, xpitch[1] = {p.M > 1 ? (unsigned long long)lda : whole};
+        const unsigned wbox[2] = {F8_BLOCK, 128}, xbox[2] = {F8_BLOCK, (unsigned)nt};
+        DABNN_REQUIRE(make_u8_tensor_map(&w_map, b, 2, wdims, wpitch, wbox) && make_u8_tensor_map(&x_map, a, 2, xdims, xpitch, xbox), DABNN_ERR_CUDA,
+                      "fp8_gemm: cannot make a tensor map (no CUDA device, or a pitch beyond 2^40)");
+    }
+    const int splits = nt <= 64 ? f8_splits(ntiles, p.nkb) : 1;
+    switch (nt) {
+        case 16: return splits > 1 ? f8_launch<16, true, T>(p, splits, w_map, x_map, stream) : f8_launch<16, false, T>(p, 1, w_map, x_map, stream);
+        case 32: return splits > 1 ? f8_launch<32, true, T>(p, splits, w_map, x_map, stream) : f8_launch<32, false, T>(p, 1, w_map, x_map, stream);
+        case 64: return splits > 1 ? f8_launch<64, true, T>(p, splits, w_map, x_map, stream) : f8_launch<64, false, T>(p, 1, w_map, x_map, stream);
+        case 128: return f8_launch<128, false, T>(p, 1, w_map, x_map, stream);
+        default: return f8_launch<256, false, T>(p, 1, w_map, x_map, stream);
+    }
+}
+
+int fp8_status_word(int** addr) {
+    DABNN_CUDA_OK(cudaGetSymbolAddress(reinterpret_cast<void**>(addr), g_fp8_status));
+    return DABNN_OK;
 }
 
 }  // namespace dabnn
@@ -114,14 +164,10 @@ extern "C" int dabnn_fp8_gemm(const uint8_t* a, long long lda, const float* a_sc
                   "fp8_gemm: rows of a and b must begin on 16-byte boundaries");
     DABNN_REQUIRE(aligned_to(c, c_type == DABNN_F32 ? 4 : 2) && aligned_to(a_scales, 4) && aligned_to(b_scales, 4) && aligned_to(bias, 4), DABNN_ERR_ARG,
                   "fp8_gemm: misaligned pointer");
+    DABNN_REQUIRE(m < INT_MAX - 512 && n < INT_MAX - 512 && k < INT_MAX - 512, DABNN_ERR_SHAPE, "fp8_gemm: too large a matrix");
     const cudaStream_t stream = static_cast<cudaStream_t>(s);
-    const dim3 grid((n + 15) / 16, (m + 15) / 16);
-    auto launch = [&](auto tag) {
-        using T = decltype(tag);
-        fp8_gemm_kernel<T><<<grid, 256, 0, stream>>>(a, lda, a_scales, as_row, as_block, b, ldb, b_scales, bs_row, bs_block, bias, static_cast<T*>(c), ldc, m, n, k);
-    };
-    if (c_type == DABNN_F32) launch(float{});
-    else if (c_type == DABNN_F16) launch(__half{});
-    else launch(__nv_bfloat16{});
-    return check_launch("fp8_gemm_kernel");
+    const Fp8Params p{a_scales, b_scales, bias, as_row, as_block, bs_row, bs_block, ldc, c, m, n};
+    if (c_type == DABNN_F32) return f8_gemm<float>(p, a, lda, b, ldb, k, stream);
+    if (c_type == DABNN_F16) return f8_gemm<__half>(p, a, lda, b, ldb, k, stream);
+    return f8_gemm<__nv_bfloat16>(p, a, lda, b, ldb, k, stream);
 }

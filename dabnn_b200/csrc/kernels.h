@@ -63,6 +63,7 @@ int bconv_u8_status(int* status);
 int contraction_status_word(int** addr);
 int fconv_status_word(int** addr);
 int bconv_u8_status_word(int** addr);
+int fp8_status_word(int** addr);   // the 8-bit float product (not part of a Net's plan)
 
 // Elementwise chain on an fp32 NHWC tensor, in one pass:  v = x;  if (a) v = a[c]*v + b[c];
 // if (add) v += add;  if (relu) v = max(v, 0);  optional fp32 store and optional sign-bit store.

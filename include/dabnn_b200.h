@@ -348,7 +348,8 @@ int dabnn_measure_tf32_peak(double* flops_per_second);
  * contraction 1 producers (a ring stage was never released), 2 epilogue (an accumulator never completed),
  * 3 / 4 MMA thread (accumulator never released / stage never filled); float convolution 11 producers, 12 epilogue, 13 / 14 MMA thread (accumulator /
  * stage), 15 / 16 row loader and its consumers; byte-activation engine 21 loader, 22 / 23 MMA thread
- * (accumulator / stage or resident weights), 24 epilogue.  A Net collects (and clears) the words itself at the
+ * (accumulator / stage or resident weights), 24 epilogue; 8-bit float product 51 loader, 52 / 53 MMA warp (accumulator /
+ * stage), 54 epilogue.  A Net collects (and clears) the words itself at the
  * end of every run and reports them as DABNN_ERR_TIMEOUT from dabnn_net_wait / _sync / _get_blob. */
 int dabnn_engine_status(int* status);
 
@@ -367,7 +368,7 @@ int dabnn_debug_set_halo(int mode);
 int dabnn_debug_set_launch_overlap(int on);
 
 /* Test hook: stores `code` in status word `which` (0 packed-bit contraction, 1 float convolution, 2 byte-activation
- * engine) exactly as a kernel whose bounded wait gave up would, so that the reporting path can be exercised
+ * engine, 3 8-bit float product) exactly as a kernel whose bounded wait gave up would, so that the reporting path can be exercised
  * without stalling a GPU. */
 int dabnn_debug_raise_engine_status(int which, int code);
 
