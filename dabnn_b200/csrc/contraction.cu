@@ -361,7 +361,7 @@ extern "C" int dabnn_engine_status(int* status) {
         const int rc = bconv_u8_status(status);
         if (rc) return rc;
     }
-    if (*status == 0) {   // the 8-bit float product (51-54)
+    if (*status == 0) {   // the 8-bit float product (51-55)
         int* word = nullptr;
         const int rc = fp8_status_word(&word);
         if (rc) return rc;

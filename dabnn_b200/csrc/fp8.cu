@@ -44,14 +44,16 @@ __global__ void __launch_bounds__(128) fp8_quantize_kernel(const T* __restrict__
     }
 }
 
+static bool aligned_to(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
 // -------------------------------------------------------------------------------------------------
-// The product: which tile, how many CTAs share one.
-static int f8_tokens_of_tile(int m, int n) {
+// The product: which tile (its columns: 16, 32, 64 activation rows or 128, 256 weight rows), how many CTAs share one.
+static int f8_columns(int m, int n) {
     if (m <= 16) return 16;
     if (m <= 32) return 32;
-    const long long tiles_n = (n + 127) / 128;
-    if (m <= 64 || tiles_n * ((m + 127) / 128) < sm_count()) return 64;
-    return tiles_n * ((m + 255) / 256) < sm_count() ? 128 : 256;
+    const long long tiles_m = ((long long)m + 127) / 128;
+    if (m <= 64 || tiles_m * ((n + 127) / 128) < sm_count()) return 64;
+    return tiles_m * ((n + 255) / 256) < sm_count() ? 128 : 256;
 }
 static int f8_splits(long long ntiles, int nkb) {
     int s = 1;
@@ -60,7 +62,7 @@ static int f8_splits(long long ntiles, int nkb) {
 }
 
 template <int NT, bool SPLIT, typename T>
-static int f8_launch(const Fp8Params& p, int splits, const CUtensorMap& w_map, const CUtensorMap& x_map, cudaStream_t stream) {
+static int f8_launch(const Fp8Params& p, int splits, const CUtensorMap& lane_map, const CUtensorMap& col_map, cudaStream_t stream) {
     using Cfg = Fp8Cfg<NT>;
     auto kern = fp8_gemm_kernel<NT, SPLIT, T>;
     static thread_local int ready_device = -1;
@@ -89,24 +91,25 @@ static int f8_launch(const Fp8Params& p, int splits, const CUtensorMap& w_map, c
     }
     cfg.attrs = attr;
     cfg.numAttrs = n;
-    DABNN_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, p, splits, w_map, x_map));
+    DABNN_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, p, splits, lane_map, col_map));
     return DABNN_OK;
 }
 
 template <typename T>
 static int f8_gemm(Fp8Params p, const uint8_t* a, long long lda, const uint8_t* b, long long ldb, int k, cudaStream_t stream) {
-    const int nt = f8_tokens_of_tile(p.M, p.N);
-    p.tiles_n = (p.N + 127) / 128;
-    const long long ntiles = (long long)p.tiles_n * ((p.M + nt - 1) / nt);
+    const int nt = f8_columns(p.M, p.N), rows_m = nt <= 64 ? nt : 128, rows_n = nt <= 64 ? 128 : nt;
+    p.tiles_n = (p.N + rows_n - 1) / rows_n;
+    const long long ntiles = (long long)p.tiles_n * ((p.M + rows_m - 1) / rows_m);
     DABNN_REQUIRE(ntiles < (1ll << 30), DABNN_ERR_SHAPE, "fp8_gemm: too many outputs");
     p.ntiles = (int)ntiles;
     p.nkb = (k + F8_BLOCK - 1) / F8_BLOCK;
+    p.vec = aligned_to(p.c, 32) && (p.M == 1 || p.ldc * sizeof(T) % 32 == 0);
     CUtensorMap w_map{}, x_map{};
     if (k > 0) {   // a single row's pitch is of no account, but the descriptor wants one
         const unsigned long long whole = ((unsigned long long)k + 15) / 16 * 16;
         const unsigned long long wdims[2] = {(unsigned long long)k, (unsigned long long)p.N}, wpitch[1] = {p.N > 1 ? (unsigned long long)ldb : whole};
         const unsigned long long xdims[2] = {(unsigned long long)k, (unsigned long long)p.M}, xpitch[1] = {p.M > 1 ? (unsigned long long)lda : whole};
-        const unsigned wbox[2] = {F8_BLOCK, 128}, xbox[2] = {F8_BLOCK, (unsigned)nt};
+        const unsigned wbox[2] = {F8_BLOCK, (unsigned)rows_n}, xbox[2] = {F8_BLOCK, (unsigned)rows_m};
         DABNN_REQUIRE(make_u8_tensor_map(&w_map, b, 2, wdims, wpitch, wbox) && make_u8_tensor_map(&x_map, a, 2, xdims, xpitch, xbox), DABNN_ERR_CUDA,
                       "fp8_gemm: cannot make a tensor map (no CUDA device, or a pitch beyond 2^40)");
     }
@@ -115,8 +118,8 @@ static int f8_gemm(Fp8Params p, const uint8_t* a, long long lda, const uint8_t* 
         case 16: return splits > 1 ? f8_launch<16, true, T>(p, splits, w_map, x_map, stream) : f8_launch<16, false, T>(p, 1, w_map, x_map, stream);
         case 32: return splits > 1 ? f8_launch<32, true, T>(p, splits, w_map, x_map, stream) : f8_launch<32, false, T>(p, 1, w_map, x_map, stream);
         case 64: return splits > 1 ? f8_launch<64, true, T>(p, splits, w_map, x_map, stream) : f8_launch<64, false, T>(p, 1, w_map, x_map, stream);
-        case 128: return f8_launch<128, false, T>(p, 1, w_map, x_map, stream);
-        default: return f8_launch<256, false, T>(p, 1, w_map, x_map, stream);
+        case 128: return f8_launch<128, false, T>(p, 1, x_map, w_map, stream);
+        default: return f8_launch<256, false, T>(p, 1, x_map, w_map, stream);
     }
 }
 
@@ -128,8 +131,6 @@ int fp8_status_word(int** addr) {
 }  // namespace dabnn
 
 using namespace dabnn;
-
-static bool aligned_to(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
 extern "C" int dabnn_fp8_quantize(const void* in, int in_type, long long ld_in, uint8_t* out, long long ld_out, float* scales, long long scale_row,
                                   long long scale_block, int rows, int k, int block_rows, dabnn_stream_t s) {

@@ -2,21 +2,22 @@
 //
 //   c[i][j] = sum over blocks q of 128 along K of as(i, q) bs(j / 128, q) sum_{h in q} a[i][h] b[j][h]   (+ bias[j])
 //
-// The weights b are the M = 128 operand and the activations a the N operand (16 .. 256 columns), so an accumulator holds 128
-// outputs (lanes) of each activation row (columns):
-//   * a tile's 128 weight rows are one block of scales: bs is one number per tile and block of K, as one per column;
-//   * few activation rows fill narrow instructions instead of an eighth of a wide one;
-//   * a warp's 32 lanes hold 32 neighbouring outputs of a row, so results go to memory straight from registers, coalesced.
 // A block of K is four instructions into one of two accumulators.  The epilogue warps read it while the other one fills,
 // multiply by as * bs and add to fp32 sums in their registers (one fused multiply-add per value and block): the tensor core's
-// own additions never run over more than 128 products.
+// own additions never run over more than 128 products.  Which operand takes the accumulator's 128 lanes and which its columns:
+//   * many rows (FEW = false): lanes are activation rows, columns weight rows.  A thread has one as, a warp one bs per block:
+//     the factor is one register, and reading the accumulator is all that passes through the shared-memory pipe.
+//   * few rows (FEW): lanes are weight rows, columns 16 .. 64 activation rows, so that they fill a narrow instruction instead of
+//     an eighth of a wide one.  The factors differ by column and come from shared memory.  A tile's 128 weight rows are one
+//     block of scales.  Few rows leave few tiles: a cluster then shares a tile (SPLIT), each CTA with a run of K's blocks, and
+//     adds up the parts over distributed shared memory in a fixed order.
 //
 // Warps: 0 TMA loads (128-byte-swizzled boxes of 128 bytes of K; rows and bytes beyond the matrices read as zeros), 1 MMA
-// issue, then the epilogue.  Few rows leave few tiles: a cluster then shares a tile, each CTA with a run of K's blocks, and
-// adds up the parts over distributed shared memory in a fixed order.
+// issue, 2 factors (scales of any strides, fetched four blocks at a time, their products left in a ring in shared memory: an
+// epilogue that fetched its own waited for them, 8192 x 8192 x 4096 in 294 us), then the epilogue.
 //
 // Every wait on an mbarrier is bounded; one that gives up records a code (51 loader, 52 / 53 MMA warp waiting for an
-// accumulator / a stage, 54 epilogue), raises the CTA's abort flag, and the CTA frees its tensor memory and returns.
+// accumulator / a stage, 54 epilogue, 55 factors), raises the CTA's abort flag, and the CTA frees its tensor memory and returns.
 #pragma once
 #include "bcontract_tc5.cuh"
 #include "scalar_types.cuh"
@@ -24,30 +25,54 @@
 namespace dabnn {
 
 constexpr int F8_BLOCK = 128;
-constexpr int F8_W_BYTES = 128 * F8_BLOCK;            // the weights of a stage
+constexpr int F8_L_BYTES = 128 * F8_BLOCK;            // the lane operand of a stage
 constexpr int F8_MAX_SPLIT = 8;
+constexpr int F8_SLOTS = 8, F8_AHEAD = 4;             // blocks of factors in the ring, blocks fetched together
 
-__device__ int g_fp8_status;   // 0 = ok; 51 - 54 as above
+__device__ int g_fp8_status;   // 0 = ok; 51 - 55 as above
 
 struct Fp8Params {
     const float *as, *bs, *bias;
     long long as_row, as_block, bs_row, bs_block, ldc;
     void* c;
     int M, N, nkb;                                     // activation rows, weight rows, blocks of K
-    int tiles_n, ntiles;                               // tiles of 128 weight rows; all tiles
+    int tiles_n, ntiles;                               // tiles along the weight rows; all tiles
+    int vec;                                           // rows of c begin on 32-byte boundaries
 };
 
 template <int NT>
-struct Fp8Cfg {                                        // NT: activation rows of a tile
-    static constexpr int EPI_WARPS = NT <= 64 ? 4 : 8;
-    static constexpr int THREADS = 64 + EPI_WARPS * 32;
+struct Fp8Cfg {                                        // NT: columns of a tile
+    static constexpr bool FEW = NT <= 64;
+    static constexpr int EPI_WARPS = FEW ? 4 : NT / 16;
+    static constexpr int EPI_WARP0 = 3, THREADS = (EPI_WARP0 + EPI_WARPS) * 32;
     static constexpr int COLS = NT / (EPI_WARPS / 4);  // accumulator columns of an epilogue warp
-    static constexpr int STAGE_BYTES = F8_W_BYTES + NT * F8_BLOCK;
+    static constexpr int FACTORS = NT;      // of a block: one per column / per lane and 128 columns
+    static constexpr int STAGE_BYTES = F8_L_BYTES + NT * F8_BLOCK;
     static constexpr int STAGES = NT <= 32 ? 5 : NT == 64 ? 4 : NT == 128 ? 6 : 4;
-    static constexpr int CTAS_PER_SM = NT <= 64 ? 2 : 1;
+    static constexpr int CTAS_PER_SM = FEW ? 2 : 1;
     static constexpr int SMEM = 1024 + STAGES * STAGE_BYTES;
 };
 
+// A bounded wait of a whole warp.  The first poll, which mostly succeeds, is all that is laid into the caller's loop.
+__device__ __noinline__ bool f8_wait_slow(uint32_t bar, uint32_t parity, const volatile int* abort_flag) {
+    for (uint32_t it = 0; it < TC5_SPIN_LIMIT; it++) {
+        uint32_t done;
+        asm volatile("{\n\t.reg .pred P1;\n\tmbarrier.try_wait.parity.shared::cta.b64 P1, [%1], %2;\n\tselp.b32 %0, 1, 0, P1;\n\t}"
+                     : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+        if (__all_sync(0xffffffffu, done)) return true;
+        if ((it & 255u) == 255u && __any_sync(0xffffffffu, *abort_flag)) return false;
+    }
+    return false;
+}
+__device__ __forceinline__ bool f8_wait(uint32_t bar, uint32_t parity, const volatile int* abort_flag) {
+    uint32_t done;
+    asm volatile("{\n\t.reg .pred P1;\n\tmbarrier.try_wait.parity.shared::cta.b64 P1, [%1], %2;\n\tselp.b32 %0, 1, 0, P1;\n\t}"
+                 : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+    return __all_sync(0xffffffffu, done) || f8_wait_slow(bar, parity, abort_flag);
+}
+__device__ __forceinline__ void f8_arrive(uint32_t bar) {
+    asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.shared::cta.b64 st, [%0];\n\t}" ::"r"(bar) : "memory");
+}
 __device__ __forceinline__ void f8_mma(uint32_t d_tmem, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t accum) {
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
                  "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}\n"
@@ -66,6 +91,11 @@ __device__ __forceinline__ void f8_tmem_ld16(uint32_t (&v)[16], uint32_t at) {
                  : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
                    "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]) : "r"(at));
 }
+// two fused multiply-adds: (x, y) += (a, b) * (sx, sy)
+__device__ __forceinline__ void f8_fma2(float2& sum, uint32_t a, uint32_t b, float sx, float sy) {
+    asm("{\n\t.reg .b64 s, v, c;\n\tmov.b64 s, {%0, %1};\n\tmov.b64 v, {%2, %3};\n\tmov.b64 c, {%4, %5};\n\t"
+        "fma.rn.f32x2 s, v, c, s;\n\tmov.b64 {%0, %1}, s;\n\t}" : "+f"(sum.x), "+f"(sum.y) : "r"(a), "r"(b), "f"(sx), "f"(sy));
+}
 __device__ __forceinline__ void f8_tmem_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ float f8_ld_cluster(uint32_t addr, int rank) {
     uint32_t remote;
@@ -81,11 +111,13 @@ __device__ __forceinline__ void f8_cluster_sync() {
 // SPLIT: the CTAs of a cluster share one tile (the grid then has one cluster per tile); otherwise a CTA walks the tiles
 template <int NT, bool SPLIT, typename T>
 __global__ void __launch_bounds__(Fp8Cfg<NT>::THREADS, Fp8Cfg<NT>::CTAS_PER_SM)
-    fp8_gemm_kernel(const Fp8Params p, const int splits, const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map) {
+    fp8_gemm_kernel(const Fp8Params p, const int splits, const __grid_constant__ CUtensorMap lane_map, const __grid_constant__ CUtensorMap col_map) {
     using Cfg = Fp8Cfg<NT>;
     extern __shared__ unsigned char smem_dyn[];
     __shared__ __align__(8) uint64_t bar_full[Cfg::STAGES], bar_empty[Cfg::STAGES], bar_acc_full[2], bar_acc_empty[2];
-    __shared__ __align__(16) float scale_s[Cfg::EPI_WARPS][Cfg::COLS];
+    __shared__ __align__(8) uint64_t bar_factor_full[F8_SLOTS], bar_factor_empty[F8_SLOTS];
+    __shared__ __align__(16) float factors[F8_SLOTS][Cfg::FACTORS];
+    __shared__ __align__(32) float scratch[Cfg::FEW ? 1 : Cfg::EPI_WARPS][32 * 8];   // to turn 32 rows of 32 bytes over, for rows of c off a boundary
     __shared__ uint32_t tmem_base_s;
     __shared__ int s_abort;
 
@@ -102,6 +134,7 @@ __global__ void __launch_bounds__(Fp8Cfg<NT>::THREADS, Fp8Cfg<NT>::CTAS_PER_SM)
     }
     if (threadIdx.x == 0) {
         for (int i = 0; i < Cfg::STAGES; i++) { mbar_init(&bar_full[i], 1); mbar_init(&bar_empty[i], 1); }
+        for (int i = 0; i < F8_SLOTS; i++) { mbar_init(&bar_factor_full[i], 1); mbar_init(&bar_factor_empty[i], Cfg::EPI_WARPS); }
         for (int i = 0; i < 2; i++) { mbar_init(&bar_acc_full[i], 1); mbar_init(&bar_acc_empty[i], Cfg::EPI_WARPS); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::);
         s_abort = 0;
@@ -129,8 +162,8 @@ __global__ void __launch_bounds__(Fp8Cfg<NT>::THREADS, Fp8Cfg<NT>::CTAS_PER_SM)
                     }
                     const uint32_t bar = smem_u32(&bar_full[s]), at = stage0 + s * Cfg::STAGE_BYTES;
                     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(Cfg::STAGE_BYTES) : "memory");
-                    f8_load(at, &w_map, kb * F8_BLOCK, tn * 128, bar);
-                    f8_load(at + F8_W_BYTES, &x_map, kb * F8_BLOCK, tm * NT, bar);
+                    f8_load(at, &lane_map, kb * F8_BLOCK, (Cfg::FEW ? tn : tm) * 128, bar);
+                    f8_load(at + F8_L_BYTES, &col_map, kb * F8_BLOCK, (Cfg::FEW ? tm : tn) * NT, bar);
                     if (++s == Cfg::STAGES) { s = 0; use++; }
                 }
             }
@@ -158,98 +191,177 @@ __global__ void __launch_bounds__(Fp8Cfg<NT>::THREADS, Fp8Cfg<NT>::CTAS_PER_SM)
                     break;
                 }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint64_t w = f8_desc(stage0 + s * Cfg::STAGE_BYTES), x = w + (F8_W_BYTES >> 4);
+                const uint64_t l = f8_desc(stage0 + s * Cfg::STAGE_BYTES), c = l + (F8_L_BYTES >> 4);
                 if (leader) {
 #pragma unroll
-                    for (int j = 0; j < F8_BLOCK / 32; j++) f8_mma(tmem_base + acc * NT, w + 2 * j, x + 2 * j, idesc, j > 0);
+                    for (int j = 0; j < F8_BLOCK / 32; j++) f8_mma(tmem_base + acc * NT, l + 2 * j, c + 2 * j, idesc, j > 0);
                     umma_commit(&bar_empty[s]);
                     umma_commit(&bar_acc_full[acc]);
                 }
                 __syncwarp();
                 if (++s == Cfg::STAGES) { s = 0; par ^= 1u; }
             }
-    } else {
-        // =========================== epilogue ===========================
-        const int ew = warp - 2, quarter = warp & 3, col0 = (ew >> 2) * Cfg::COLS;   // TMEM lane quarter of a warp = warp % 4
-        const uint32_t t_mine = tmem_base + ((uint32_t)(quarter * 32) << 16) + col0;
-        float* const my_scales = scale_s[ew];
-        constexpr int SC = (Cfg::COLS + 31) / 32;      // scales that a lane fetches
+    } else if (warp == 2) {
+        // =========================== factors as * bs ===========================
+        // FEW: a lane has the columns lane, lane + 32; else rows lane + 32 j of the tile, each with the bs of every 128 columns
+        constexpr int MINE = Cfg::FEW ? (NT + 31) / 32 : 4, BLOCKS = Cfg::FEW ? 1 : NT / 128;
         int i = 0;
         bool ok = true;
         for (int tile = first; tile < p.ntiles && ok; tile += step) {
             const int tm = tile / p.tiles_n, tn = tile - tm * p.tiles_n;
-            const int m0 = tm * NT + col0;
-            float sum[Cfg::COLS];
+            const int m0 = tm * (Cfg::FEW ? NT : 128) + lane;
+            const float* a[MINE];
+            const float* b[BLOCKS];
 #pragma unroll
-            for (int e = 0; e < Cfg::COLS; e++) sum[e] = 0.f;
-            // the scales of a block, fetched two blocks ahead
-            float next[2][SC], wnext[2];
-            auto fetch = [&](int kb, float (&v)[SC], float& w) {
-                w = kb < kb1 ? __ldg(p.bs + tn * p.bs_row + kb * p.bs_block) : 0.f;
+            for (int e = 0; e < MINE; e++) a[e] = p.as + min(m0 + e * 32, p.M - 1) * p.as_row;
 #pragma unroll
-                for (int e = 0; e < SC; e++) {
-                    const int m = m0 + e * 32 + lane;
-                    v[e] = kb < kb1 && m < p.M && e * 32 + lane < Cfg::COLS ? __ldg(p.as + m * p.as_row + kb * p.as_block) : 0.f;
+            for (int e = 0; e < BLOCKS; e++) b[e] = p.bs + min(tn * BLOCKS + e, (p.N - 1) >> 7) * p.bs_row;
+            for (int kb = kb0; kb < kb1 && ok; kb += F8_AHEAD) {
+                float av[F8_AHEAD][MINE], bv[F8_AHEAD][BLOCKS];
+#pragma unroll
+                for (int g = 0; g < F8_AHEAD; g++) {
+                    const long long q = min(kb + g, kb1 - 1);
+#pragma unroll
+                    for (int e = 0; e < MINE; e++) av[g][e] = __ldg(a[e] + q * p.as_block);
+#pragma unroll
+                    for (int e = 0; e < BLOCKS; e++) bv[g][e] = __ldg(b[e] + q * p.bs_block);
                 }
-            };
-            fetch(kb0, next[0], wnext[0]);
-            fetch(kb0 + 1, next[1], wnext[1]);
-            for (int kb = kb0; kb < kb1; kb++, i++) {
-                __syncwarp();                          // the scales of the block before have been read
 #pragma unroll
-                for (int e = 0; e < SC; e++)
-                    if (e * 32 + lane < Cfg::COLS) my_scales[e * 32 + lane] = next[0][e] * wnext[0];
+                for (int g = 0; g < F8_AHEAD; g++) {
+                    if (kb + g >= kb1) break;
+                    const int slot = i % F8_SLOTS;
+                    if (i >= F8_SLOTS && !mbar_wait_warp(&bar_factor_empty[slot], (i / F8_SLOTS - 1) & 1, abort_flag)) {
+                        atomicCAS(&g_fp8_status, 0, 55);
+                        s_abort = 1;
+                        ok = false;
+                        break;
+                    }
 #pragma unroll
-                for (int e = 0; e < SC; e++) next[0][e] = next[1][e];
-                wnext[0] = wnext[1];
-                fetch(kb + 2, next[1], wnext[1]);
-                __syncwarp();
-                const int acc = i & 1;
-                if (!mbar_wait_warp(&bar_acc_full[acc], (i >> 1) & 1, abort_flag)) {
+                    for (int e = 0; e < MINE; e++)
+#pragma unroll
+                        for (int h = 0; h < BLOCKS; h++)
+                            if (!Cfg::FEW || e * 32 + lane < NT) factors[slot][h * 128 + e * 32 + lane] = av[g][e] * bv[g][h];
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&bar_factor_full[slot]);
+                    i++;
+                }
+            }
+        }
+    } else {
+        // =========================== epilogue ===========================
+        const int ew = warp - Cfg::EPI_WARP0, quarter = warp & 3, col0 = (ew >> 2) * Cfg::COLS;   // TMEM lane quarter of a warp = warp % 4
+        const uint32_t t_mine = tmem_base + ((uint32_t)(quarter * 32) << 16) + col0;
+        // Walking state: one accumulator and one slot of factors further with every block.  The sums and one chunk of an
+        // accumulator take 80 of the 96 registers that 19 warps leave; two chunks, and addresses were recomputed in every block
+        // (8192 x 8192 x 4096: 294 us).
+        uint32_t slot = 0, slot_par = 0, acc = 0, acc_par = 0;
+        const uint32_t acc_full = smem_u32(bar_acc_full), acc_empty = smem_u32(bar_acc_empty), factor_full = smem_u32(bar_factor_full),
+                       factor_empty = smem_u32(bar_factor_empty);
+        const uint32_t my_factors = smem_u32(factors) + (Cfg::FEW ? col0 : (col0 & ~127) + quarter * 32 + lane) * 4;
+        bool ok = true;
+        for (int tile = first; tile < p.ntiles && ok; tile += step) {
+            float2 sum[Cfg::COLS / 2];
+#pragma unroll
+            for (int e = 0; e < Cfg::COLS / 2; e++) sum[e] = make_float2(0.f, 0.f);
+            auto sum_of = [&](int e) { return e & 1 ? sum[e >> 1].y : sum[e >> 1].x; };
+#pragma unroll 1
+            for (int left = kb1 - kb0; left > 0; left--) {
+                if (!f8_wait(factor_full + slot * 8, slot_par, abort_flag) || !f8_wait(acc_full + acc * 8, acc_par, abort_flag)) {
                     atomicCAS(&g_fp8_status, 0, 54);
                     s_abort = 1;
                     ok = false;
                     break;
                 }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                uint32_t v[2][16];
-                f8_tmem_ld16(v[0], t_mine + acc * NT);
+                constexpr int CHUNKS = Cfg::COLS / 16;
+                const uint32_t t_acc = t_mine + acc * NT, mine = my_factors + slot * (Cfg::FACTORS * 4);
+                uint32_t v[16];
+                f8_tmem_ld16(v, t_acc);
+                const float factor = Cfg::FEW ? 0.f : lds_f32(mine);
 #pragma unroll
-                for (int h = 0; h < Cfg::COLS / 16; h++) {
+                for (int h = 0; h < CHUNKS; h++) {
                     f8_tmem_wait();
-                    if (h + 1 < Cfg::COLS / 16) {
-                        f8_tmem_ld16(v[(h + 1) & 1], t_mine + acc * NT + (h + 1) * 16);
-                    } else {                           // all of it is in registers: the MMA warp may reuse the accumulator
+                    if (h == CHUNKS - 1) {             // all of it is in registers: the MMA warp may reuse the accumulator
                         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&bar_acc_empty[acc]);
+                        if (elect_lane()) f8_arrive(acc_empty + acc * 8);
                     }
 #pragma unroll
                     for (int e = 0; e < 16; e += 4) {
-                        const float4 sc = lds128f(smem_u32(my_scales + h * 16 + e));
-                        sum[h * 16 + e] = fmaf(__uint_as_float(v[h & 1][e]), sc.x, sum[h * 16 + e]);
-                        sum[h * 16 + e + 1] = fmaf(__uint_as_float(v[h & 1][e + 1]), sc.y, sum[h * 16 + e + 1]);
-                        sum[h * 16 + e + 2] = fmaf(__uint_as_float(v[h & 1][e + 2]), sc.z, sum[h * 16 + e + 2]);
-                        sum[h * 16 + e + 3] = fmaf(__uint_as_float(v[h & 1][e + 3]), sc.w, sum[h * 16 + e + 3]);
+                        const float4 sc = Cfg::FEW ? lds128f(mine + (h * 16 + e) * 4) : make_float4(factor, factor, factor, factor);
+                        f8_fma2(sum[(h * 16 + e) / 2], v[e], v[e + 1], sc.x, sc.y);
+                        f8_fma2(sum[(h * 16 + e) / 2 + 1], v[e + 2], v[e + 3], sc.z, sc.w);
                     }
+                    if (h + 1 < CHUNKS) f8_tmem_ld16(v, t_acc + (h + 1) * 16);
                 }
+                __syncwarp();
+                if (elect_lane()) f8_arrive(factor_empty + slot * 8);
+                if (++slot == F8_SLOTS) { slot = 0; slot_par ^= 1; }
+                acc ^= 1;
+                if (!acc) acc_par ^= 1;
             }
+            if (!ok) break;
+            const int tm = tile / p.tiles_n, tn = tile - tm * p.tiles_n;
+            const int m0 = Cfg::FEW ? tm * NT + col0 : tm * 128 + quarter * 32;   // first activation row and output of the warp
+            const int n0 = Cfg::FEW ? tn * 128 + quarter * 32 : tn * NT + col0;
             if (SPLIT) {
                 // this CTA's part -> its shared memory (the ring is idle: its last loads have been multiplied), [column][output]
                 const uint32_t part = stage0 + (uint32_t)((col0 * 128 + quarter * 32 + lane) * 4);
-                if (ok)
 #pragma unroll
-                    for (int e = 0; e < Cfg::COLS; e++) asm volatile("st.shared.f32 [%0], %1;" ::"r"(part + e * 512), "f"(sum[e]) : "memory");
-            } else if (ok) {
-                const int n = tn * 128 + quarter * 32 + lane;
+                for (int e = 0; e < Cfg::COLS; e++) asm volatile("st.shared.f32 [%0], %1;" ::"r"(part + e * 512), "f"(sum_of(e)) : "memory");
+            } else if (Cfg::FEW) {
+                // a warp's lanes are neighbouring outputs of a row
+                const int n = n0 + lane;
                 if (n < p.N) {
                     const float bias = p.bias ? __ldg(p.bias + n) : 0.f;
                     T* out = static_cast<T*>(p.c) + m0 * p.ldc + n;
                     const int left = p.M - m0;
 #pragma unroll
                     for (int e = 0; e < Cfg::COLS; e++) {
-                        if (e < left) *out = from_f32<T>(sum[e] + bias);
+                        if (e < left) *out = from_f32<T>(sum_of(e) + bias);
                         out += p.ldc;
+                    }
+                }
+            } else {
+                // a thread has neighbouring outputs of its row: 32 bytes at a time
+                constexpr int W = 32 / (int)sizeof(T);
+                const int m = m0 + lane;
+                T* const out = static_cast<T*>(p.c) + m * p.ldc + n0;
+                if (p.bias) {                          // through shared memory: a warp's columns are the same in all its lanes
+                    const uint32_t mine = smem_u32(scratch[ew]);
+                    __syncwarp();
+#pragma unroll
+                    for (int e = 0; e < Cfg::COLS; e += 32) scratch[ew][e + lane] = __ldg(p.bias + min(n0 + e + lane, p.N - 1));
+                    __syncwarp();
+#pragma unroll
+                    for (int e = 0; e < Cfg::COLS; e += 4) {
+                        const float4 b = lds128f(mine + e * 4);
+                        sum[e / 2].x += b.x; sum[e / 2].y += b.y; sum[e / 2 + 1].x += b.z; sum[e / 2 + 1].y += b.w;
+                    }
+                }
+#pragma unroll
+                for (int h = 0; h < Cfg::COLS; h += W) {
+                    const int left = p.N - n0 - h;     // the same in all lanes
+                    if (left <= 0) break;
+                    alignas(32) T o[W];
+#pragma unroll
+                    for (int e = 0; e < W; e++) o[e] = from_f32<T>(sum_of(h + e));
+                    const uint4 *lo = reinterpret_cast<const uint4*>(o), *hi = lo + 1;
+                    if (p.vec && left >= W) {
+                        if (m < p.M)
+                            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out + h), "r"(lo->x), "r"(lo->y), "r"(lo->z),
+                                         "r"(lo->w), "r"(hi->x), "r"(hi->y), "r"(hi->z), "r"(hi->w) : "memory");
+                    } else {                           // turned over, so that W lanes write neighbouring outputs of a row
+                        __syncwarp();
+                        const uint32_t mine = smem_u32(scratch[ew]);
+                        sts128(mine + lane * 32, lo->x, lo->y, lo->z, lo->w);
+                        sts128(mine + lane * 32 + 16, hi->x, hi->y, hi->z, hi->w);
+                        __syncwarp();
+                        const T* turned = reinterpret_cast<const T*>(scratch[ew]);
+#pragma unroll
+                        for (int q = 0; q < W; q++) {
+                            const int r = q * (32 / W) + lane / W, e = lane % W;
+                            if (m0 + r < p.M && e < left) static_cast<T*>(p.c)[(m0 + r) * p.ldc + n0 + h + e] = turned[r * W + e];
+                        }
                     }
                 }
             }

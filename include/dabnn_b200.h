@@ -349,7 +349,7 @@ int dabnn_measure_tf32_peak(double* flops_per_second);
  * 3 / 4 MMA thread (accumulator never released / stage never filled); float convolution 11 producers, 12 epilogue, 13 / 14 MMA thread (accumulator /
  * stage), 15 / 16 row loader and its consumers; byte-activation engine 21 loader, 22 / 23 MMA thread
  * (accumulator / stage or resident weights), 24 epilogue; 8-bit float product 51 loader, 52 / 53 MMA warp (accumulator /
- * stage), 54 epilogue.  A Net collects (and clears) the words itself at the
+ * stage), 54 epilogue, 55 factors.  A Net collects (and clears) the words itself at the
  * end of every run and reports them as DABNN_ERR_TIMEOUT from dabnn_net_wait / _sync / _get_blob. */
 int dabnn_engine_status(int* status);
 
