@@ -51,9 +51,8 @@ static bool aligned_to(const void* p, size_t bytes) { return (reinterpret_cast<u
 static int f8_columns(int m, int n) {
     if (m <= 16) return 16;
     if (m <= 32) return 32;
-    const long long tiles_m = ((long long)m + 127) / 128;
-    if (m <= 64 || tiles_m * ((n + 127) / 128) < sm_count()) return 64;
-    return tiles_m * ((n + 255) / 256) < sm_count() ? 128 : 256;
+    if (m <= 64 || ((long long)m + 127) / 128 * ((n + 127) / 128) < sm_count()) return 64;
+    return ((long long)m + 255) / 256 * ((n + 255) / 256) < sm_count() / 2 ? 128 : 256;
 }
 static int f8_splits(long long ntiles, int nkb) {
     int s = 1;
@@ -65,31 +64,39 @@ template <int NT, bool SPLIT, typename T>
 static int f8_launch(const Fp8Params& p, int splits, const CUtensorMap& lane_map, const CUtensorMap& col_map, cudaStream_t stream) {
     using Cfg = Fp8Cfg<NT>;
     auto kern = fp8_gemm_kernel<NT, SPLIT, T>;
-    static thread_local int ready_device = -1;
+    static thread_local int ready_device = -1, resident = 0;   // teams that run at once
     int dev = 0;
     DABNN_CUDA_OK(cudaGetDevice(&dev));
     if (dev != ready_device) {
         DABNN_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM));
-        ready_device = dev;
     }
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(SPLIT ? p.ntiles * splits : std::min(p.ntiles, sm_count() * Cfg::CTAS_PER_SM));
+    const int team = SPLIT ? splits : Cfg::PAIR ? 2 : 1;
     cfg.blockDim = dim3(Cfg::THREADS);
     cfg.dynamicSmemBytes = Cfg::SMEM;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
+    cfg.attrs = attr;
     int n = 0;
+    if (team > 1) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = team;
+        attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+        n++;
+    }
+    cfg.numAttrs = n;
+    cfg.gridDim = dim3(team);
+    if (dev != ready_device) {
+        if (Cfg::PAIR) DABNN_CUDA_OK(cudaOccupancyMaxActiveClusters(&resident, kern, &cfg));
+        else resident = sm_count() * Cfg::CTAS_PER_SM;
+        DABNN_REQUIRE(resident > 0, DABNN_ERR_CUDA, "fp8_gemm: the device runs no pair of CTAs");
+        ready_device = dev;
+    }
+    cfg.gridDim = dim3((SPLIT ? p.ntiles : std::min(p.ntiles, resident)) * team);
     if (g_overlap_launches) {
         attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr[n++].val.programmaticStreamSerializationAllowed = 1;
     }
-    if (SPLIT) {
-        attr[n].id = cudaLaunchAttributeClusterDimension;
-        attr[n].val.clusterDim.x = splits;
-        attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
-        n++;
-    }
-    cfg.attrs = attr;
     cfg.numAttrs = n;
     DABNN_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, p, splits, lane_map, col_map));
     return DABNN_OK;
@@ -97,7 +104,7 @@ static int f8_launch(const Fp8Params& p, int splits, const CUtensorMap& lane_map
 
 template <typename T>
 static int f8_gemm(Fp8Params p, const uint8_t* a, long long lda, const uint8_t* b, long long ldb, int k, cudaStream_t stream) {
-    const int nt = f8_columns(p.M, p.N), rows_m = nt <= 64 ? nt : 128, rows_n = nt <= 64 ? 128 : nt;
+    const int nt = f8_columns(p.M, p.N), rows_m = nt <= 64 ? nt : nt == 128 ? 128 : 256, rows_n = nt <= 64 ? 128 : nt;
     p.tiles_n = (p.N + rows_n - 1) / rows_n;
     const long long ntiles = (long long)p.tiles_n * ((p.M + rows_m - 1) / rows_m);
     DABNN_REQUIRE(ntiles < (1ll << 30), DABNN_ERR_SHAPE, "fp8_gemm: too many outputs");
@@ -109,7 +116,7 @@ static int f8_gemm(Fp8Params p, const uint8_t* a, long long lda, const uint8_t* 
         const unsigned long long whole = ((unsigned long long)k + 15) / 16 * 16;
         const unsigned long long wdims[2] = {(unsigned long long)k, (unsigned long long)p.N}, wpitch[1] = {p.N > 1 ? (unsigned long long)ldb : whole};
         const unsigned long long xdims[2] = {(unsigned long long)k, (unsigned long long)p.M}, xpitch[1] = {p.M > 1 ? (unsigned long long)lda : whole};
-        const unsigned wbox[2] = {F8_BLOCK, (unsigned)rows_n}, xbox[2] = {F8_BLOCK, (unsigned)rows_m};
+        const unsigned wbox[2] = {F8_BLOCK, (unsigned)std::min(rows_n, 128)}, xbox[2] = {F8_BLOCK, (unsigned)std::min(rows_m, 128)};   // (a pair loads halves)
         DABNN_REQUIRE(make_u8_tensor_map(&w_map, b, 2, wdims, wpitch, wbox) && make_u8_tensor_map(&x_map, a, 2, xdims, xpitch, xbox), DABNN_ERR_CUDA,
                       "fp8_gemm: cannot make a tensor map (no CUDA device, or a pitch beyond 2^40)");
     }

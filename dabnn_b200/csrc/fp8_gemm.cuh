@@ -27,7 +27,7 @@ namespace dabnn {
 constexpr int F8_BLOCK = 128;
 constexpr int F8_L_BYTES = 128 * F8_BLOCK;            // the lane operand of a stage
 constexpr int F8_MAX_SPLIT = 8;
-constexpr int F8_SLOTS = 8, F8_AHEAD = 4;             // blocks of factors in the ring, blocks fetched together
+constexpr int F8_GROUPS = 2, F8_GROUP = 4;            // the ring of factors: groups of blocks, fetched and handed over together
 
 __device__ int g_fp8_status;   // 0 = ok; 51 - 55 as above
 
@@ -42,13 +42,14 @@ struct Fp8Params {
 
 template <int NT>
 struct Fp8Cfg {                                        // NT: columns of a tile
-    static constexpr bool FEW = NT <= 64;
+    static constexpr bool FEW = NT <= 64, PAIR = NT == 256;
     static constexpr int EPI_WARPS = FEW ? 4 : NT / 16;
     static constexpr int EPI_WARP0 = 3, THREADS = (EPI_WARP0 + EPI_WARPS) * 32;
     static constexpr int COLS = NT / (EPI_WARPS / 4);  // accumulator columns of an epilogue warp
     static constexpr int FACTORS = NT;      // of a block: one per column / per lane and 128 columns
-    static constexpr int STAGE_BYTES = F8_L_BYTES + NT * F8_BLOCK;
-    static constexpr int STAGES = NT <= 32 ? 5 : NT == 64 ? 4 : NT == 128 ? 6 : 4;
+    static constexpr int COL_ROWS = PAIR ? NT / 2 : NT;  // rows of the column operand that a CTA loads
+    static constexpr int STAGE_BYTES = F8_L_BYTES + COL_ROWS * F8_BLOCK;
+    static constexpr int STAGES = NT <= 32 ? 5 : NT == 64 ? 4 : 6;
     static constexpr int CTAS_PER_SM = FEW ? 2 : 1;
     static constexpr int SMEM = 1024 + STAGES * STAGE_BYTES;
 };
@@ -73,17 +74,43 @@ __device__ __forceinline__ bool f8_wait(uint32_t bar, uint32_t parity, const vol
 __device__ __forceinline__ void f8_arrive(uint32_t bar) {
     asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.shared::cta.b64 st, [%0];\n\t}" ::"r"(bar) : "memory");
 }
+template <bool PAIR>
 __device__ __forceinline__ void f8_mma(uint32_t d_tmem, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t accum) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}\n"
-                 ::"r"(d_tmem), "l"(ad), "l"(bd), "r"(idesc), "r"(accum), "r"(0), "r"(0), "r"(0), "r"(0) : "memory");
+    if (PAIR)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n"
+                     ::"r"(d_tmem), "l"(ad), "l"(bd), "r"(idesc), "r"(accum) : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n"
+                     ::"r"(d_tmem), "l"(ad), "l"(bd), "r"(idesc), "r"(accum) : "memory");
+}
+// the barrier of this CTA, or those at the same place in both CTAs of the pair
+template <bool PAIR>
+__device__ __forceinline__ void f8_commit(uint32_t bar) {
+    if (PAIR)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((unsigned short)3) : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ uint32_t f8_in_cta(uint32_t addr, int rank) {   // the same place in another CTA of the cluster
+    uint32_t there;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(addr), "r"(rank));
+    return there;
+}
+// (relaxed: what it follows are loads from tensor memory that have been waited for; a release across the cluster takes hundreds of cycles)
+__device__ __forceinline__ void f8_arrive_cluster(uint32_t bar) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 // K-major SWIZZLE_128B: rows of 128 bytes, 8-row groups 1024 bytes apart
 __device__ __forceinline__ uint64_t f8_desc(uint32_t saddr) {
     return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
+template <bool PAIR>
 __device__ __forceinline__ void f8_load(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+    if (PAIR)   // the barrier may be the other CTA's
+        asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                     ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar) : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
                  ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar) : "memory");
 }
 __device__ __forceinline__ void f8_tmem_ld16(uint32_t (&v)[16], uint32_t at) {
@@ -98,10 +125,8 @@ __device__ __forceinline__ void f8_fma2(float2& sum, uint32_t a, uint32_t b, flo
 }
 __device__ __forceinline__ void f8_tmem_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ float f8_ld_cluster(uint32_t addr, int rank) {
-    uint32_t remote;
     float v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(f8_in_cta(addr, rank)) : "memory");
     return v;
 }
 __device__ __forceinline__ void f8_cluster_sync() {
@@ -115,8 +140,8 @@ __global__ void __launch_bounds__(Fp8Cfg<NT>::THREADS, Fp8Cfg<NT>::CTAS_PER_SM)
     using Cfg = Fp8Cfg<NT>;
     extern __shared__ unsigned char smem_dyn[];
     __shared__ __align__(8) uint64_t bar_full[Cfg::STAGES], bar_empty[Cfg::STAGES], bar_acc_full[2], bar_acc_empty[2];
-    __shared__ __align__(8) uint64_t bar_factor_full[F8_SLOTS], bar_factor_empty[F8_SLOTS];
-    __shared__ __align__(16) float factors[F8_SLOTS][Cfg::FACTORS];
+    __shared__ __align__(8) uint64_t bar_factor_full[F8_GROUPS], bar_factor_empty[F8_GROUPS];
+    __shared__ __align__(16) float factors[F8_GROUPS][F8_GROUP][Cfg::FACTORS];
     __shared__ __align__(32) float scratch[Cfg::FEW ? 1 : Cfg::EPI_WARPS][32 * 8];   // to turn 32 rows of 32 bytes over, for rows of c off a boundary
     __shared__ uint32_t tmem_base_s;
     __shared__ int s_abort;
@@ -125,22 +150,30 @@ __global__ void __launch_bounds__(Fp8Cfg<NT>::THREADS, Fp8Cfg<NT>::CTAS_PER_SM)
     const uint32_t stage0 = (smem_u32(smem_dyn) + 1023u) & ~1023u;
     const volatile int* abort_flag = &s_abort;
     constexpr int TMEM_COLS = 2 * NT;
-    const int rank = SPLIT ? (int)blockIdx.x % splits : 0, first = SPLIT ? (int)blockIdx.x / splits : (int)blockIdx.x, step = SPLIT ? p.ntiles : (int)gridDim.x;
+    constexpr bool PAIR = Cfg::PAIR;
+    const int team = SPLIT ? splits : PAIR ? 2 : 1;    // CTAs that share a tile: the cluster
+    const int rank = (int)blockIdx.x % team, first = (int)blockIdx.x / team, step = (int)gridDim.x / team;
     const int kb0 = SPLIT ? (int)((long long)p.nkb * rank / splits) : 0, kb1 = SPLIT ? (int)((long long)p.nkb * (rank + 1) / splits) : p.nkb;
 
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_s)), "r"(TMEM_COLS));
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+        if (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_s)), "r"(TMEM_COLS));
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_s)), "r"(TMEM_COLS));
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+        }
     }
     if (threadIdx.x == 0) {
         for (int i = 0; i < Cfg::STAGES; i++) { mbar_init(&bar_full[i], 1); mbar_init(&bar_empty[i], 1); }
-        for (int i = 0; i < F8_SLOTS; i++) { mbar_init(&bar_factor_full[i], 1); mbar_init(&bar_factor_empty[i], Cfg::EPI_WARPS); }
-        for (int i = 0; i < 2; i++) { mbar_init(&bar_acc_full[i], 1); mbar_init(&bar_acc_empty[i], Cfg::EPI_WARPS); }
+        for (int i = 0; i < F8_GROUPS; i++) { mbar_init(&bar_factor_full[i], 1); mbar_init(&bar_factor_empty[i], Cfg::EPI_WARPS); }
+        for (int i = 0; i < 2; i++) { mbar_init(&bar_acc_full[i], 1); mbar_init(&bar_acc_empty[i], (PAIR ? 2 : 1) * Cfg::EPI_WARPS); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::);
         s_abort = 0;
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    if (PAIR) f8_cluster_sync();                       // the other CTA's barriers are set up
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem_base = tmem_base_s;
     grid_launch_dependents();
@@ -160,31 +193,34 @@ __global__ void __launch_bounds__(Fp8Cfg<NT>::THREADS, Fp8Cfg<NT>::CTAS_PER_SM)
                         ok = false;
                         break;
                     }
-                    const uint32_t bar = smem_u32(&bar_full[s]), at = stage0 + s * Cfg::STAGE_BYTES;
-                    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(Cfg::STAGE_BYTES) : "memory");
-                    f8_load(at, &lane_map, kb * F8_BLOCK, (Cfg::FEW ? tn : tm) * 128, bar);
-                    f8_load(at + F8_L_BYTES, &col_map, kb * F8_BLOCK, (Cfg::FEW ? tm : tn) * NT, bar);
+                    const uint32_t at = stage0 + s * Cfg::STAGE_BYTES;
+                    uint32_t bar = smem_u32(&bar_full[s]);
+                    if (!PAIR || rank == 0)
+                        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"((PAIR ? 2 : 1) * Cfg::STAGE_BYTES) : "memory");
+                    if (PAIR) bar = f8_in_cta(bar, 0);   // the CTA that issues for both waits for both
+                    f8_load<PAIR>(at, &lane_map, kb * F8_BLOCK, (Cfg::FEW ? tn : PAIR ? tm * 2 + rank : tm) * 128, bar);
+                    f8_load<PAIR>(at + F8_L_BYTES, &col_map, kb * F8_BLOCK, (Cfg::FEW ? tm : tn) * NT + (PAIR ? rank * Cfg::COL_ROWS : 0), bar);
                     if (++s == Cfg::STAGES) { s = 0; use++; }
                 }
             }
         }
     } else if (warp == 1) {
-        // =========================== MMA issue: the whole warp walks, one lane issues ===========================
+        // =========================== MMA issue: the whole warp walks, one lane issues, for a pair the first CTA's ===========================
         const bool leader = elect_lane();
-        constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(NT >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);   // D f32, A = B = e4m3, K-major
+        constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(NT >> 3) << 17) | ((uint32_t)((PAIR ? 256 : 128) >> 4) << 24);   // D f32, A = B = e4m3, K-major
         uint32_t s = 0, par = 0;
-        bool ok = true;
+        bool ok = !PAIR || rank == 0;
         int i = 0;   // blocks so far
         for (int tile = first; tile < p.ntiles && ok; tile += step)
             for (int kb = kb0; kb < kb1; kb++, i++) {
                 const int acc = i & 1;
-                if (i >= 2 && !mbar_wait_warp(&bar_acc_empty[acc], ((i >> 1) - 1) & 1, abort_flag)) {
+                if (i >= 2 && !f8_wait(smem_u32(&bar_acc_empty[acc]), ((i >> 1) - 1) & 1, abort_flag)) {
                     atomicCAS(&g_fp8_status, 0, 52);
                     s_abort = 1;
                     ok = false;
                     break;
                 }
-                if (!mbar_wait_warp(&bar_full[s], par, abort_flag)) {
+                if (!f8_wait(smem_u32(&bar_full[s]), par, abort_flag)) {
                     atomicCAS(&g_fp8_status, 0, 53);
                     s_abort = 1;
                     ok = false;
@@ -194,9 +230,9 @@ __global__ void __launch_bounds__(Fp8Cfg<NT>::THREADS, Fp8Cfg<NT>::CTAS_PER_SM)
                 const uint64_t l = f8_desc(stage0 + s * Cfg::STAGE_BYTES), c = l + (F8_L_BYTES >> 4);
                 if (leader) {
 #pragma unroll
-                    for (int j = 0; j < F8_BLOCK / 32; j++) f8_mma(tmem_base + acc * NT, l + 2 * j, c + 2 * j, idesc, j > 0);
-                    umma_commit(&bar_empty[s]);
-                    umma_commit(&bar_acc_full[acc]);
+                    for (int j = 0; j < F8_BLOCK / 32; j++) f8_mma<PAIR>(tmem_base + acc * NT, l + 2 * j, c + 2 * j, idesc, j > 0);
+                    f8_commit<PAIR>(smem_u32(&bar_empty[s]));
+                    f8_commit<PAIR>(smem_u32(&bar_acc_full[acc]));
                 }
                 __syncwarp();
                 if (++s == Cfg::STAGES) { s = 0; par ^= 1u; }
@@ -209,53 +245,50 @@ __global__ void __launch_bounds__(Fp8Cfg<NT>::THREADS, Fp8Cfg<NT>::CTAS_PER_SM)
         bool ok = true;
         for (int tile = first; tile < p.ntiles && ok; tile += step) {
             const int tm = tile / p.tiles_n, tn = tile - tm * p.tiles_n;
-            const int m0 = tm * (Cfg::FEW ? NT : 128) + lane;
+            const int m0 = (Cfg::FEW ? tm * NT : (PAIR ? tm * 2 + rank : tm) * 128) + lane;
             const float* a[MINE];
             const float* b[BLOCKS];
 #pragma unroll
             for (int e = 0; e < MINE; e++) a[e] = p.as + min(m0 + e * 32, p.M - 1) * p.as_row;
 #pragma unroll
             for (int e = 0; e < BLOCKS; e++) b[e] = p.bs + min(tn * BLOCKS + e, (p.N - 1) >> 7) * p.bs_row;
-            for (int kb = kb0; kb < kb1 && ok; kb += F8_AHEAD) {
-                float av[F8_AHEAD][MINE], bv[F8_AHEAD][BLOCKS];
+            for (int kb = kb0; kb < kb1; kb += F8_GROUP, i++) {   // (a tile begins with a new group)
+                float av[F8_GROUP][MINE], bv[F8_GROUP][BLOCKS];
 #pragma unroll
-                for (int g = 0; g < F8_AHEAD; g++) {
+                for (int g = 0; g < F8_GROUP; g++) {
                     const long long q = min(kb + g, kb1 - 1);
 #pragma unroll
                     for (int e = 0; e < MINE; e++) av[g][e] = __ldg(a[e] + q * p.as_block);
 #pragma unroll
                     for (int e = 0; e < BLOCKS; e++) bv[g][e] = __ldg(b[e] + q * p.bs_block);
                 }
+                const int slot = i % F8_GROUPS;
+                if (i >= F8_GROUPS && !f8_wait(smem_u32(&bar_factor_empty[slot]), (i / F8_GROUPS - 1) & 1, abort_flag)) {
+                    atomicCAS(&g_fp8_status, 0, 55);
+                    s_abort = 1;
+                    ok = false;
+                    break;
+                }
 #pragma unroll
-                for (int g = 0; g < F8_AHEAD; g++) {
-                    if (kb + g >= kb1) break;
-                    const int slot = i % F8_SLOTS;
-                    if (i >= F8_SLOTS && !mbar_wait_warp(&bar_factor_empty[slot], (i / F8_SLOTS - 1) & 1, abort_flag)) {
-                        atomicCAS(&g_fp8_status, 0, 55);
-                        s_abort = 1;
-                        ok = false;
-                        break;
-                    }
+                for (int g = 0; g < F8_GROUP; g++)
 #pragma unroll
                     for (int e = 0; e < MINE; e++)
 #pragma unroll
                         for (int h = 0; h < BLOCKS; h++)
-                            if (!Cfg::FEW || e * 32 + lane < NT) factors[slot][h * 128 + e * 32 + lane] = av[g][e] * bv[g][h];
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&bar_factor_full[slot]);
-                    i++;
-                }
+                            if (!Cfg::FEW || e * 32 + lane < NT) factors[slot][g][h * 128 + e * 32 + lane] = av[g][e] * bv[g][h];
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bar_factor_full[slot]);
             }
         }
     } else {
         // =========================== epilogue ===========================
         const int ew = warp - Cfg::EPI_WARP0, quarter = warp & 3, col0 = (ew >> 2) * Cfg::COLS;   // TMEM lane quarter of a warp = warp % 4
         const uint32_t t_mine = tmem_base + ((uint32_t)(quarter * 32) << 16) + col0;
-        // Walking state: one accumulator and one slot of factors further with every block.  The sums and one chunk of an
+        // Walking state: one accumulator further with every block, one slot of factors with every group of them.  The sums and one chunk of an
         // accumulator take 80 of the 96 registers that 19 warps leave; two chunks, and addresses were recomputed in every block
         // (8192 x 8192 x 4096: 294 us).
         uint32_t slot = 0, slot_par = 0, acc = 0, acc_par = 0;
-        const uint32_t acc_full = smem_u32(bar_acc_full), acc_empty = smem_u32(bar_acc_empty), factor_full = smem_u32(bar_factor_full),
+        const uint32_t acc_full = smem_u32(bar_acc_full), acc_empty = PAIR ? f8_in_cta(smem_u32(bar_acc_empty), 0) : smem_u32(bar_acc_empty), factor_full = smem_u32(bar_factor_full),
                        factor_empty = smem_u32(bar_factor_empty);
         const uint32_t my_factors = smem_u32(factors) + (Cfg::FEW ? col0 : (col0 & ~127) + quarter * 32 + lane) * 4;
         bool ok = true;
@@ -264,9 +297,17 @@ __global__ void __launch_bounds__(Fp8Cfg<NT>::THREADS, Fp8Cfg<NT>::CTAS_PER_SM)
 #pragma unroll
             for (int e = 0; e < Cfg::COLS / 2; e++) sum[e] = make_float2(0.f, 0.f);
             auto sum_of = [&](int e) { return e & 1 ? sum[e >> 1].y : sum[e >> 1].x; };
+            uint32_t mine = 0;                         // this block's factors
+            int in_group = F8_GROUP;
 #pragma unroll 1
             for (int left = kb1 - kb0; left > 0; left--) {
-                if (!f8_wait(factor_full + slot * 8, slot_par, abort_flag) || !f8_wait(acc_full + acc * 8, acc_par, abort_flag)) {
+                bool there = true;
+                if (in_group == F8_GROUP) {
+                    there = f8_wait(factor_full + slot * 8, slot_par, abort_flag);
+                    mine = my_factors + slot * (F8_GROUP * Cfg::FACTORS * 4);
+                    in_group = 0;
+                }
+                if (!there || !f8_wait(acc_full + acc * 8, acc_par, abort_flag)) {
                     atomicCAS(&g_fp8_status, 0, 54);
                     s_abort = 1;
                     ok = false;
@@ -274,7 +315,7 @@ __global__ void __launch_bounds__(Fp8Cfg<NT>::THREADS, Fp8Cfg<NT>::CTAS_PER_SM)
                 }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 constexpr int CHUNKS = Cfg::COLS / 16;
-                const uint32_t t_acc = t_mine + acc * NT, mine = my_factors + slot * (Cfg::FACTORS * 4);
+                const uint32_t t_acc = t_mine + acc * NT;
                 uint32_t v[16];
                 f8_tmem_ld16(v, t_acc);
                 const float factor = Cfg::FEW ? 0.f : lds_f32(mine);
@@ -283,7 +324,10 @@ __global__ void __launch_bounds__(Fp8Cfg<NT>::THREADS, Fp8Cfg<NT>::CTAS_PER_SM)
                     f8_tmem_wait();
                     if (h == CHUNKS - 1) {             // all of it is in registers: the MMA warp may reuse the accumulator
                         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                        if (elect_lane()) f8_arrive(acc_empty + acc * 8);
+                        if (elect_lane()) {
+                            if (PAIR) f8_arrive_cluster(acc_empty + acc * 8);
+                            else f8_arrive(acc_empty + acc * 8);
+                        }
                     }
 #pragma unroll
                     for (int e = 0; e < 16; e += 4) {
@@ -293,15 +337,19 @@ __global__ void __launch_bounds__(Fp8Cfg<NT>::THREADS, Fp8Cfg<NT>::CTAS_PER_SM)
                     }
                     if (h + 1 < CHUNKS) f8_tmem_ld16(v, t_acc + (h + 1) * 16);
                 }
-                __syncwarp();
-                if (elect_lane()) f8_arrive(factor_empty + slot * 8);
-                if (++slot == F8_SLOTS) { slot = 0; slot_par ^= 1; }
+                mine += Cfg::FACTORS * 4;
+                if (++in_group == F8_GROUP || left == 1) {
+                    in_group = F8_GROUP;
+                    __syncwarp();
+                    if (elect_lane()) f8_arrive(factor_empty + slot * 8);
+                    if (++slot == F8_GROUPS) { slot = 0; slot_par ^= 1; }
+                }
                 acc ^= 1;
                 if (!acc) acc_par ^= 1;
             }
             if (!ok) break;
             const int tm = tile / p.tiles_n, tn = tile - tm * p.tiles_n;
-            const int m0 = Cfg::FEW ? tm * NT + col0 : tm * 128 + quarter * 32;   // first activation row and output of the warp
+            const int m0 = Cfg::FEW ? tm * NT + col0 : (PAIR ? tm * 2 + rank : tm) * 128 + quarter * 32;   // first activation row and output of the warp
             const int n0 = Cfg::FEW ? tn * 128 + quarter * 32 : tn * NT + col0;
             if (SPLIT) {
                 // this CTA's part -> its shared memory (the ring is idle: its last loads have been multiplied), [column][output]
@@ -389,9 +437,11 @@ __global__ void __launch_bounds__(Fp8Cfg<NT>::THREADS, Fp8Cfg<NT>::CTAS_PER_SM)
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    if (PAIR) f8_cluster_sync();                       // no CTA leaves while the other arrives at its barriers
     if (warp == 1) {
         __syncwarp();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS));
+        if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS));
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS));
     }
 }
 
