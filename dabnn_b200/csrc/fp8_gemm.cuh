@@ -44,7 +44,7 @@ template <int NT>
 struct Fp8Cfg {                                        // NT: columns of a tile
     static constexpr bool FEW = NT <= 64, PAIR = NT == 256;
     static constexpr int EPI_WARPS = FEW ? 4 : NT / 16;
-    static constexpr int EPI_WARP0 = 3, THREADS = (EPI_WARP0 + EPI_WARPS) * 32;
+    static constexpr int EPI_WARP0 = PAIR ? 4 : 3, THREADS = (EPI_WARP0 + EPI_WARPS) * 32;
     static constexpr int COLS = NT / (EPI_WARPS / 4);  // accumulator columns of an epilogue warp
     static constexpr int FACTORS = NT;      // of a block: one per column / per lane and 128 columns
     static constexpr int COL_ROWS = PAIR ? NT / 2 : NT;  // rows of the column operand that a CTA loads
@@ -54,8 +54,8 @@ struct Fp8Cfg {                                        // NT: columns of a tile
     static constexpr int SMEM = 1024 + STAGES * STAGE_BYTES;
 };
 
-// A bounded wait of a whole warp.  The first poll, which mostly succeeds, is all that is laid into the caller's loop.
-__device__ __noinline__ bool f8_wait_slow(uint32_t bar, uint32_t parity, const volatile int* abort_flag) {
+// A bounded wait of a whole warp
+__device__ __forceinline__ bool f8_wait(uint32_t bar, uint32_t parity, const volatile int* abort_flag) {
     for (uint32_t it = 0; it < TC5_SPIN_LIMIT; it++) {
         uint32_t done;
         asm volatile("{\n\t.reg .pred P1;\n\tmbarrier.try_wait.parity.shared::cta.b64 P1, [%1], %2;\n\tselp.b32 %0, 1, 0, P1;\n\t}"
@@ -64,12 +64,6 @@ __device__ __noinline__ bool f8_wait_slow(uint32_t bar, uint32_t parity, const v
         if ((it & 255u) == 255u && __any_sync(0xffffffffu, *abort_flag)) return false;
     }
     return false;
-}
-__device__ __forceinline__ bool f8_wait(uint32_t bar, uint32_t parity, const volatile int* abort_flag) {
-    uint32_t done;
-    asm volatile("{\n\t.reg .pred P1;\n\tmbarrier.try_wait.parity.shared::cta.b64 P1, [%1], %2;\n\tselp.b32 %0, 1, 0, P1;\n\t}"
-                 : "=r"(done) : "r"(bar), "r"(parity) : "memory");
-    return __all_sync(0xffffffffu, done) || f8_wait_slow(bar, parity, abort_flag);
 }
 __device__ __forceinline__ void f8_arrive(uint32_t bar) {
     asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.shared::cta.b64 st, [%0];\n\t}" ::"r"(bar) : "memory");
@@ -178,7 +172,10 @@ __global__ void __launch_bounds__(Fp8Cfg<NT>::THREADS, Fp8Cfg<NT>::CTAS_PER_SM)
     const uint32_t tmem_base = tmem_base_s;
     grid_launch_dependents();
     grid_dependency_wait();
-
+    if (warp < Cfg::EPI_WARP0) {
+    // a pair's 20 warps have 96 registers each at launch: these four give 32 of theirs to the epilogue's sixteen, whose sums and two
+    // chunks of an accumulator take 96
+    if (PAIR) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     if (warp == 0) {
         // =========================== TMA loads: one lane ===========================
         if (elect_lane()) {
@@ -246,21 +243,18 @@ __global__ void __launch_bounds__(Fp8Cfg<NT>::THREADS, Fp8Cfg<NT>::CTAS_PER_SM)
         for (int tile = first; tile < p.ntiles && ok; tile += step) {
             const int tm = tile / p.tiles_n, tn = tile - tm * p.tiles_n;
             const int m0 = (Cfg::FEW ? tm * NT : (PAIR ? tm * 2 + rank : tm) * 128) + lane;
-            const float* a[MINE];
-            const float* b[BLOCKS];
-#pragma unroll
-            for (int e = 0; e < MINE; e++) a[e] = p.as + min(m0 + e * 32, p.M - 1) * p.as_row;
-#pragma unroll
-            for (int e = 0; e < BLOCKS; e++) b[e] = p.bs + min(tn * BLOCKS + e, (p.N - 1) >> 7) * p.bs_row;
+            const float* a = p.as + m0 * p.as_row + kb0 * p.as_block;
+            const float* b = p.bs + (long long)tn * BLOCKS * p.bs_row + kb0 * p.bs_block;
             for (int kb = kb0; kb < kb1; kb += F8_GROUP, i++) {   // (a tile begins with a new group)
                 float av[F8_GROUP][MINE], bv[F8_GROUP][BLOCKS];
 #pragma unroll
                 for (int g = 0; g < F8_GROUP; g++) {
-                    const long long q = min(kb + g, kb1 - 1);
 #pragma unroll
-                    for (int e = 0; e < MINE; e++) av[g][e] = __ldg(a[e] + q * p.as_block);
+                    for (int e = 0; e < MINE; e++) av[g][e] = kb + g < kb1 && m0 + e * 32 < p.M ? __ldg(a + e * 32 * p.as_row) : 0.f;
 #pragma unroll
-                    for (int e = 0; e < BLOCKS; e++) bv[g][e] = __ldg(b[e] + q * p.bs_block);
+                    for (int e = 0; e < BLOCKS; e++) bv[g][e] = kb + g < kb1 && (tn * BLOCKS + e) * 128 < p.N ? __ldg(b + e * p.bs_row) : 0.f;
+                    a += p.as_block;
+                    b += p.bs_block;
                 }
                 const int slot = i % F8_GROUPS;
                 if (i >= F8_GROUPS && !f8_wait(smem_u32(&bar_factor_empty[slot]), (i / F8_GROUPS - 1) & 1, abort_flag)) {
@@ -280,13 +274,13 @@ __global__ void __launch_bounds__(Fp8Cfg<NT>::THREADS, Fp8Cfg<NT>::CTAS_PER_SM)
                 if (lane == 0) mbar_arrive(&bar_factor_full[slot]);
             }
         }
+    }
     } else {
         // =========================== epilogue ===========================
+        if (PAIR) asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
         const int ew = warp - Cfg::EPI_WARP0, quarter = warp & 3, col0 = (ew >> 2) * Cfg::COLS;   // TMEM lane quarter of a warp = warp % 4
         const uint32_t t_mine = tmem_base + ((uint32_t)(quarter * 32) << 16) + col0;
-        // Walking state: one accumulator further with every block, one slot of factors with every group of them.  The sums and one chunk of an
-        // accumulator take 80 of the 96 registers that 19 warps leave; two chunks, and addresses were recomputed in every block
-        // (8192 x 8192 x 4096: 294 us).
+        // Walking state: one accumulator further with every block, one slot of factors with every group of them.
         uint32_t slot = 0, slot_par = 0, acc = 0, acc_par = 0;
         const uint32_t acc_full = smem_u32(bar_acc_full), acc_empty = PAIR ? f8_in_cta(smem_u32(bar_acc_empty), 0) : smem_u32(bar_acc_empty), factor_full = smem_u32(bar_factor_full),
                        factor_empty = smem_u32(bar_factor_empty);
@@ -314,15 +308,17 @@ __global__ void __launch_bounds__(Fp8Cfg<NT>::THREADS, Fp8Cfg<NT>::CTAS_PER_SM)
                     break;
                 }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                // 16 columns at a time, two loads to a wait
                 constexpr int CHUNKS = Cfg::COLS / 16;
                 const uint32_t t_acc = t_mine + acc * NT;
-                uint32_t v[16];
-                f8_tmem_ld16(v, t_acc);
+                uint32_t v[2][16];
+                f8_tmem_ld16(v[0], t_acc);
+                if (CHUNKS > 1) f8_tmem_ld16(v[1], t_acc + 16);
                 const float factor = Cfg::FEW ? 0.f : lds_f32(mine);
 #pragma unroll
                 for (int h = 0; h < CHUNKS; h++) {
-                    f8_tmem_wait();
-                    if (h == CHUNKS - 1) {             // all of it is in registers: the MMA warp may reuse the accumulator
+                    if (h % 2 == 0) f8_tmem_wait();
+                    if (h == max(CHUNKS - 2, 0)) {     // all of it is in registers: the MMA warp may reuse the accumulator
                         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                         if (elect_lane()) {
                             if (PAIR) f8_arrive_cluster(acc_empty + acc * 8);
@@ -332,10 +328,10 @@ __global__ void __launch_bounds__(Fp8Cfg<NT>::THREADS, Fp8Cfg<NT>::CTAS_PER_SM)
 #pragma unroll
                     for (int e = 0; e < 16; e += 4) {
                         const float4 sc = Cfg::FEW ? lds128f(mine + (h * 16 + e) * 4) : make_float4(factor, factor, factor, factor);
-                        f8_fma2(sum[(h * 16 + e) / 2], v[e], v[e + 1], sc.x, sc.y);
-                        f8_fma2(sum[(h * 16 + e) / 2 + 1], v[e + 2], v[e + 3], sc.z, sc.w);
+                        f8_fma2(sum[(h * 16 + e) / 2], v[h & 1][e], v[h & 1][e + 1], sc.x, sc.y);
+                        f8_fma2(sum[(h * 16 + e) / 2 + 1], v[h & 1][e + 2], v[h & 1][e + 3], sc.z, sc.w);
                     }
-                    if (h + 1 < CHUNKS) f8_tmem_ld16(v, t_acc + (h + 1) * 16);
+                    if (h + 2 < CHUNKS) f8_tmem_ld16(v[h & 1], t_acc + (h + 2) * 16);
                 }
                 mine += Cfg::FACTORS * 4;
                 if (++in_group == F8_GROUP || left == 1) {
