@@ -3,45 +3,182 @@
 
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 #include "fp8_gemm.cuh"
 #include "kernels.h"
 
 namespace dabnn {
 
-// The scale of a block whose largest finite magnitude has the bits `top` (fp32): the least power of two 2^e, e >= -126, with
-// top <= 448 * 2^e, 448 = 1.75 * 2^8 being the largest e4m3 value.  As bits; the reciprocal's bits are (254 << 23) - scale.
+// -------------------------------------------------------------------------------------------------
+// The quantiser: per block, A = the largest finite |x|, scale = 2^e with e = max(-126, least integer with A <= 448 * 2^e),
+// q = e4m3(x * 2^-e).  A power of two, so that the product is exact, the rounding to e4m3 the only one, and a block's values
+// the same whichever order or width they are computed in; 8-bit floats lose nothing by it but the lowest binade.
+// One pass over the data: a thread keeps its values in registers between the maximum and the conversion.  Bound by HBM.
+
+// the scale's bits from those of A (fp32), 448 = 1.75 * 2^8; the reciprocal's bits are (254 << 23) - scale
 __device__ __forceinline__ uint32_t f8_scale_bits(uint32_t top) {
     const int e = (int)(top >> 23) - 127 - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
     return (uint32_t)(max(e, -126) + 127) << 23;
 }
 
-// one CTA per block of block_rows x 128
+// 16 neighbouring values of a row, as they lie in memory
 template <typename T>
-__global__ void __launch_bounds__(128) fp8_quantize_kernel(const T* __restrict__ in, const long long ld_in, uint8_t* __restrict__ out, const long long ld_out,
-                                                           float* __restrict__ scales, const long long scale_row, const long long scale_block,
-                                                           const int rows, const int k, const int block_rows) {
-    __shared__ uint32_t top_s;
-    const int kb = blockIdx.y, col = kb * F8_BLOCK + threadIdx.x;
-    const long long r0 = (long long)blockIdx.x * block_rows;
-    const int nr = (int)min((long long)block_rows, rows - r0);
-    if (threadIdx.x == 0) top_s = 0;
-    __syncthreads();
-    uint32_t top = 0;
-    for (int r = 0; r < nr && col < k; r++) {
-        const uint32_t a = __float_as_uint(to_f32(in[(r0 + r) * ld_in + col])) & 0x7fffffffu;
-        if (a < 0x7f800000u) top = max(top, a);
+struct Sixteen {
+    static constexpr int WORDS = 16 * sizeof(T) / 4;
+    uint32_t w[WORDS];
+
+    __device__ __forceinline__ void load(const T* at, int left, bool vec) {   // left: values before the row's end; the others read as zeros
+        if (left >= 16 && vec) {
+#pragma unroll
+            for (int i = 0; i < WORDS; i += 4) {
+                const uint4 v = __ldg(reinterpret_cast<const uint4*>(at) + i / 4);
+                w[i] = v.x; w[i + 1] = v.y; w[i + 2] = v.z; w[i + 3] = v.w;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < WORDS; i++) w[i] = 0;
+#pragma unroll
+            for (int i = 0; i < 16; i++)
+                if (i < left) {
+                    if constexpr (sizeof(T) == 4) w[i] = __ldg(reinterpret_cast<const uint32_t*>(at) + i);
+                    else w[i / 2] |= (uint32_t)__ldg(reinterpret_cast<const unsigned short*>(at) + i) << (i % 2 * 16);
+                }
+        }
     }
-    atomicMax(&top_s, top);
-    __syncthreads();
-    const uint32_t scale = f8_scale_bits(top_s);
-    const float inv = __uint_as_float((254u << 23) - scale);
-    if (threadIdx.x == 0) scales[blockIdx.x * scale_row + kb * scale_block] = __uint_as_float(scale);
-    for (int r = 0; r < nr && col < k; r++) {
-        const float x = to_f32(in[(r0 + r) * ld_in + col]);
-        const bool finite = (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u;
-        out[(r0 + r) * ld_out + col] = finite ? __nv_cvt_float_to_fp8(x * inv, __NV_SATFINITE, __NV_E4M3) : 0x7f;
+    __device__ __forceinline__ float value(int i) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+        else if constexpr (std::is_same_v<T, __nv_bfloat16>) return __uint_as_float(i % 2 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+        else return __half2float(__ushort_as_half((unsigned short)(w[i / 2] >> (i % 2 * 16))));
     }
+    // fp32 bits of the largest magnitude; an infinity or a NaN counts (>= 0x7f800000), or with finite = true is passed over
+    __device__ __forceinline__ uint32_t top(bool finite) const {
+        uint32_t m = 0;
+        if (finite) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const uint32_t a = __float_as_uint(value(i)) & 0x7fffffffu;
+                if (a < 0x7f800000u) m = max(m, a);
+            }
+            return m;
+        }
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < WORDS; i++) m = max(m, w[i] & 0x7fffffffu);
+            return m;
+        } else {   // two at a time: the order of magnitudes is that of their bits
+#pragma unroll
+            for (int i = 0; i < WORDS; i++) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+            const unsigned short s = (unsigned short)max(m & 0xffffu, m >> 16);
+            if constexpr (std::is_same_v<T, __nv_bfloat16>) return (uint32_t)s << 16;
+            else return __float_as_uint(__half2float(__ushort_as_half(s)));
+        }
+    }
+    __device__ __forceinline__ uint4 bytes(float inv, bool special) const {
+        uint32_t o[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(value(4 * i) * inv, value(4 * i + 1) * inv), __NV_SATFINITE, __NV_E4M3);
+            const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(value(4 * i + 2) * inv, value(4 * i + 3) * inv), __NV_SATFINITE, __NV_E4M3);
+            o[i] = lo | hi << 16;
+        }
+        if (special) {   // the conversion makes infinities the largest value
+#pragma unroll
+            for (int i = 0; i < 16; i++)
+                if ((__float_as_uint(value(i)) & 0x7f800000u) == 0x7f800000u) o[i / 4] |= 0x7fu << (i % 4 * 8);
+        }
+        return make_uint4(o[0], o[1], o[2], o[3]);
+    }
+};
+
+__device__ __forceinline__ void f8_store16(uint8_t* at, uint4 v, int left, bool vec) {
+    if (left >= 16 && vec) {
+        *reinterpret_cast<uint4*>(at) = v;
+    } else {
+        const uint32_t o[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 16; i++)
+            if (i < left) at[i] = (uint8_t)(o[i / 4] >> (i % 4 * 8));
+    }
+}
+
+// Blocks of one row.  Eight lanes a block, 16 values each; a warp has 2^kshift neighbouring blocks of 4 >> kshift rows (four
+// of one row unless rows have fewer), a CTA eight warps' rows, whose scales it writes side by side.
+constexpr int FQ_WARPS = 8;
+template <typename T>
+__global__ void __launch_bounds__(FQ_WARPS * 32) fp8_quantize_rows_kernel(const T* __restrict__ in, const long long ld_in, uint8_t* __restrict__ out,
+                                                                          const long long ld_out, float* __restrict__ scales, const long long scale_row,
+                                                                          const long long scale_block, const int rows, const int k, const int kshift,
+                                                                          const int kgroups, const int vec_in, const int vec_out) {
+    __shared__ float scale_s[FQ_WARPS * 4];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, unit = lane >> 3;
+    const int rows_warp = 4 >> kshift;
+    const int kb = ((int)(blockIdx.x % kgroups) << kshift) + (unit & ((1 << kshift) - 1));
+    const long long row0 = (long long)(blockIdx.x / kgroups) * (FQ_WARPS * rows_warp);
+    const int r = warp * rows_warp + (unit >> kshift);
+    const long long row = row0 + r;
+    const int col = kb * F8_BLOCK + (lane & 7) * 16, left = row < rows ? k - col : 0;
+    grid_dependency_wait();
+
+    Sixteen<T> v;
+    v.load(in + row * ld_in + col, left, vec_in);
+    auto eight = [](uint32_t m) {
+#pragma unroll
+        for (int d = 1; d < 8; d <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
+        return m;
+    };
+    uint32_t top = eight(v.top(false));
+    const bool special = top >= 0x7f800000u;
+    if (__any_sync(0xffffffffu, special)) top = eight(v.top(true));
+    const uint32_t scale = f8_scale_bits(top);
+    if (left > 0) f8_store16(out + row * ld_out + col, v.bytes(__uint_as_float((254u << 23) - scale), special), left, vec_out);
+    if ((lane & 7) == 0) scale_s[(unit & ((1 << kshift) - 1)) * (FQ_WARPS * rows_warp) + r] = __uint_as_float(scale);
+    __syncthreads();
+    if (threadIdx.x < FQ_WARPS * 4) {
+        const int b = threadIdx.x / (FQ_WARPS * rows_warp), rr = threadIdx.x % (FQ_WARPS * rows_warp);
+        const long long q = ((long long)(blockIdx.x % kgroups) << kshift) + b;
+        if (row0 + rr < rows && q * F8_BLOCK < k) scales[(row0 + rr) * scale_row + q * scale_block] = scale_s[threadIdx.x];
+    }
+}
+
+// Blocks of 128 x 128, one CTA each: 64 values of a thread, of four rows
+template <typename T>
+__global__ void __launch_bounds__(256) fp8_quantize_blocks_kernel(const T* __restrict__ in, const long long ld_in, uint8_t* __restrict__ out, const long long ld_out,
+                                                                  float* __restrict__ scales, const long long scale_row, const long long scale_block,
+                                                                  const int rows, const int k, const int kblocks, const int vec_in, const int vec_out) {
+    __shared__ uint32_t top_s[2][8];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int kb = blockIdx.x % kblocks, rb = blockIdx.x / kblocks;
+    const int col = kb * F8_BLOCK + (threadIdx.x & 7) * 16;
+    const long long row = (long long)rb * F8_BLOCK + (threadIdx.x >> 3);
+    grid_dependency_wait();
+
+    Sixteen<T> v[4];
+    int left[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        left[j] = row + j * 32 < rows ? k - col : 0;
+        v[j].load(in + (row + j * 32) * ld_in + col, left[j], vec_in);
+    }
+    auto all = [&](bool finite, uint32_t* shared) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int j = 0; j < 4; j++) m = max(m, v[j].top(finite));
+        m = __reduce_max_sync(0xffffffffu, m);
+        if (lane == 0) shared[warp] = m;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 8; i++) m = max(m, shared[i]);
+        return m;
+    };
+    uint32_t top = all(false, top_s[0]);
+    const bool special = top >= 0x7f800000u;
+    if (special) top = all(true, top_s[1]);
+    const uint32_t scale = f8_scale_bits(top);
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+        if (left[j] > 0) f8_store16(out + (row + j * 32) * ld_out + col, v[j].bytes(__uint_as_float((254u << 23) - scale), special), left[j], vec_out);
+    if (threadIdx.x == 0) scales[rb * scale_row + kb * scale_block] = __uint_as_float(scale);
 }
 
 static bool aligned_to(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
@@ -143,21 +280,35 @@ extern "C" int dabnn_fp8_quantize(const void* in, int in_type, long long ld_in, 
                                   long long scale_block, int rows, int k, int block_rows, dabnn_stream_t s) {
     DABNN_REQUIRE(in_type >= DABNN_F32 && in_type <= DABNN_BF16, DABNN_ERR_ARG, "fp8_quantize: unknown input type");
     DABNN_REQUIRE(rows >= 0 && k >= 0, DABNN_ERR_ARG, "fp8_quantize: bad dims");
+    DABNN_REQUIRE(k < INT_MAX - 512, DABNN_ERR_SHAPE, "fp8_quantize: too large a matrix");
     DABNN_REQUIRE(block_rows == 1 || block_rows == F8_BLOCK, DABNN_ERR_ARG, "fp8_quantize: a scale's block has 1 or 128 rows");
     if (rows == 0 || k == 0) return DABNN_OK;
     DABNN_REQUIRE(in && out && scales, DABNN_ERR_ARG, "fp8_quantize: null pointer");
     DABNN_REQUIRE(ld_in >= k && ld_out >= k, DABNN_ERR_SHAPE, "fp8_quantize: a row pitch is below k");
     DABNN_REQUIRE(aligned_to(in, in_type == DABNN_F32 ? 4 : 2) && aligned_to(scales, 4), DABNN_ERR_ARG, "fp8_quantize: misaligned pointer");
     const cudaStream_t stream = static_cast<cudaStream_t>(s);
-    const dim3 grid((rows + block_rows - 1) / block_rows, (k + F8_BLOCK - 1) / F8_BLOCK);
-    auto launch = [&](auto tag) {
+    auto launch = [&](auto tag) -> int {
         using T = decltype(tag);
-        fp8_quantize_kernel<T><<<grid, 128, 0, stream>>>(static_cast<const T*>(in), ld_in, out, ld_out, scales, scale_row, scale_block, rows, k, block_rows);
+        const T* x = static_cast<const T*>(in);
+        const int vec_in = aligned_to(in, 16) && (rows == 1 || ld_in * sizeof(T) % 16 == 0), vec_out = aligned_to(out, 16) && (rows == 1 || ld_out % 16 == 0);
+        const long long kblocks = ((long long)k + F8_BLOCK - 1) / F8_BLOCK;
+        if (block_rows == 1) {
+            const int kshift = kblocks >= 4 ? 2 : kblocks >= 2 ? 1 : 0, rows_cta = FQ_WARPS * (4 >> kshift);
+            const long long kgroups = (kblocks + (1 << kshift) - 1) >> kshift, ctas = kgroups * (((long long)rows + rows_cta - 1) / rows_cta);
+            DABNN_REQUIRE(ctas < INT_MAX, DABNN_ERR_SHAPE, "fp8_quantize: too large a matrix");
+            DABNN_CUDA_OK(launch_overlapped(fp8_quantize_rows_kernel<T>, dim3((unsigned)ctas), dim3(FQ_WARPS * 32), 0, stream, x, ld_in, out, ld_out, scales, scale_row,
+                                            scale_block, rows, k, kshift, (int)kgroups, vec_in, vec_out));
+        } else {
+            const long long ctas = kblocks * (((long long)rows + F8_BLOCK - 1) / F8_BLOCK);
+            DABNN_REQUIRE(ctas < INT_MAX, DABNN_ERR_SHAPE, "fp8_quantize: too large a matrix");
+            DABNN_CUDA_OK(launch_overlapped(fp8_quantize_blocks_kernel<T>, dim3((unsigned)ctas), dim3(256), 0, stream, x, ld_in, out, ld_out, scales, scale_row,
+                                            scale_block, rows, k, (int)kblocks, vec_in, vec_out));
+        }
+        return DABNN_OK;
     };
-    if (in_type == DABNN_F32) launch(float{});
-    else if (in_type == DABNN_F16) launch(__half{});
-    else launch(__nv_bfloat16{});
-    return check_launch("fp8_quantize_kernel");
+    if (in_type == DABNN_F32) return launch(float{});
+    if (in_type == DABNN_F16) return launch(__half{});
+    return launch(__nv_bfloat16{});
 }
 
 extern "C" int dabnn_fp8_gemm(const uint8_t* a, long long lda, const float* a_scales, long long as_row, long long as_block, const uint8_t* b,

@@ -4,7 +4,19 @@
 //   log p_j = d_j - ln S,   entropy = -sum p ln p = ln S - W / S
 //
 // Classes are ordered by value, larger first, equal ones (the two zeros are) by index, a NaN before everything.
+//
+// One pass over a row, no lane waiting for another: a lane keeps its own m, S, W (rescaled when its m grows) and its own count
+// of classes before the label; a warp keeps its best classes in order, one to a lane.  A batch of a warp - 64 bytes of each
+// lane - is looked at for alternatives only if some lane's maximum passes the warp's threshold (its k-th best, or another
+// warp's of the row), which after a row's first batches is rare.  What it finds goes through a queue in shared memory and is
+// inserted one by one.  The first batch has no threshold yet: the k-th largest of the 64 half-lane maxima is one, since there are
+// then at least k classes that reach it.
+//
+// A row is scored by one warp, or by a CTA of eight, or by a cluster of such CTAs where rows are few: the warps take the row's
+// batches in turn and their parts are joined at the end, lists of best classes by counting, for each entry, the better ones.
+#include <algorithm>
 #include <climits>
+#include <type_traits>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -12,85 +24,440 @@
 
 namespace dabnn {
 
-// fp32 -> unsigned, order preserved; a NaN is the largest, the zeros are one value
+constexpr int LP_WARPS = 8, LP_MAX_CLUSTER = 8;
+constexpr float LP_LOG2E = 1.4426950408889634f, LP_LN2 = 0.6931471805599453f;
+constexpr float LP_FLOOR = -1e30f;                     // a difference below it has e^d = 0; keeps d e^d a number
+
+// fp32 -> unsigned, order preserved; a NaN is the largest, the zeros are one value, nothing is 0
 __device__ __forceinline__ uint32_t order_key(float x) {
     const uint32_t u = __float_as_uint(x + 0.f);
     if (x != x) return 0xffffffffu;
     return u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float key_value(uint32_t key) {
-    return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
+    return key == 0xffffffffu ? __int_as_float(0x7fc00000) : __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
+}
+// t with: not (v <= t) exactly where v's key is at least `key` (for the key of -inf t is a NaN, which all pass)
+__device__ __forceinline__ float pass_from(uint32_t key) {
+    if (key == 0xffffffffu) return INFINITY;           // NaN alone
+    const uint32_t below = key - (key == 0x80000000u ? 2 : 1);
+    return __uint_as_float(below & 0x80000000u ? below ^ 0x80000000u : ~below);
+}
+// t with: not (v <= t) exactly where v's key is above `key`
+__device__ __forceinline__ float pass_above(uint32_t key) { return key == 0xffffffffu ? INFINITY : pass_from(key + 1); }
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float exp2_fast(float x) {   // ex2.approx: off by 2^-22
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
 }
 
-template <typename V, typename F>
-__device__ V block_reduce(V v, F op, V* shared) {
-    shared[threadIdx.x] = v;
-    __syncthreads();
-    for (int n = blockDim.x / 2; n; n >>= 1) {
-        if ((int)threadIdx.x < n) shared[threadIdx.x] = op(shared[threadIdx.x], shared[threadIdx.x + n]);
-        __syncthreads();
+// Part of a row: its maximum, and S and W relative to it, W in units of ln 2 (the argument that ex2 wants anyway)
+struct Part {
+    float m, s, w;
+    __device__ __forceinline__ void raise(float to) {   // to >= m
+        const float delta = m == -INFINITY ? 0.f : fminf((to - m) * LP_LOG2E, -LP_FLOOR), scale = exp2_fast(-delta);
+        w = scale * (w - delta * s);
+        s *= scale;
+        m = to;
     }
-    v = shared[0];
-    __syncthreads();
-    return v;
-}
+    __device__ __forceinline__ void join(Part o) {
+        const float to = fmaxf(m, o.m);
+        raise(to);
+        o.raise(to);
+        s += o.s;
+        w += o.w;
+    }
+};
 
-// one CTA per row
 template <typename T>
-__global__ void __launch_bounds__(256) logprobs_kernel(const T* __restrict__ logits, const long long ld, const int64_t* __restrict__ labels, const int classes,
-                                                       float* label_logprob, int64_t* label_rank, float* entropy, float* top_logprob,
-                                                       int64_t* top_index, const int top) {
-    __shared__ float fs[256];
-    __shared__ unsigned long long us[256];
-    const long long row = blockIdx.x;
-    const T* x = logits + row * ld;
-    auto maxu = [](unsigned long long a, unsigned long long b) { return a > b ? a : b; };
-    auto add = [](float a, float b) { return a + b; };
-    float m = -INFINITY;
-    for (int j = threadIdx.x; j < classes; j += 256) m = fmaxf(m, to_f32(x[j]));
-    m = block_reduce(m, [](float a, float b) { return fmaxf(a, b); }, fs);
-    const int64_t label = labels ? labels[row] : -1;
-    const bool have = label >= 0 && label < classes;
-    const float mine = have ? to_f32(x[label]) : 0.f;
+struct Vec {                                           // 16 bytes of a row
+    static constexpr int N = 16 / (int)sizeof(T);
+    uint4 raw;
+    __device__ __forceinline__ float value(int i) const {
+        const uint32_t w = sizeof(T) == 4 ? (i == 0 ? raw.x : i == 1 ? raw.y : i == 2 ? raw.z : raw.w) : (i < 2 ? raw.x : i < 4 ? raw.y : i < 6 ? raw.z : raw.w);
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w);
+        else if constexpr (std::is_same_v<T, __nv_bfloat16>) return __uint_as_float(i % 2 ? w & 0xffff0000u : w << 16);
+        else return __half2float(__ushort_as_half((unsigned short)(i % 2 ? w >> 16 : w)));
+    }
+    // values at [first, first + N) of a row of n, -inf outside it; `row` + first is on a 16-byte boundary
+    __device__ __forceinline__ void load(const T* row, int first, int n) {
+        if (first >= 0 && first + N <= n) {
+            raw = __ldg(reinterpret_cast<const uint4*>(row + first));
+            return;
+        }
+        uint32_t w[4];
+        constexpr uint32_t NONE = sizeof(T) == 4 ? 0xff800000u : std::is_same_v<T, __nv_bfloat16> ? 0xff80ff80u : 0xfc00fc00u;
+        w[0] = w[1] = w[2] = w[3] = NONE;
+#pragma unroll
+        for (int i = 0; i < N; i++)
+            if (first + i >= 0 && first + i < n) {
+                if constexpr (sizeof(T) == 4) w[i] = __ldg(reinterpret_cast<const uint32_t*>(row) + first + i);
+                else {
+                    const uint32_t v = __ldg(reinterpret_cast<const unsigned short*>(row) + first + i);
+                    w[i / 2] = i % 2 ? (w[i / 2] & 0xffffu) | v << 16 : (w[i / 2] & 0xffff0000u) | v;
+                }
+            }
+        raw = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+};
+
+// The best classes of a warp so far, in order: entry lane (and, with two, lane + 32) is key << 32 | ~index; 0: none yet
+template <int ENTRIES>
+struct Best {
+    unsigned long long e[ENTRIES == 0 ? 1 : ENTRIES];
+    __device__ __forceinline__ void insert(unsigned long long x) {   // x: the same in all lanes
+        const int lane = threadIdx.x & 31;
+        int pos = 0;
+#pragma unroll
+        for (int h = 0; h < ENTRIES; h++) pos += __popc(__ballot_sync(0xffffffffu, e[h] > x));
+        unsigned long long carry = 0;
+#pragma unroll
+        for (int h = 0; h < ENTRIES; h++) {
+            const unsigned long long up = __shfl_up_sync(0xffffffffu, e[h], 1), last = __shfl_sync(0xffffffffu, e[h], 31);
+            const int at = h * 32 + lane;
+            if (at > pos) e[h] = lane ? up : carry;
+            else if (at == pos) e[h] = x;
+            carry = last;
+        }
+    }
+    __device__ __forceinline__ unsigned long long at(int i) const {   // i: the same in all lanes
+        unsigned long long x = __shfl_sync(0xffffffffu, e[0], i & 31);
+        if (ENTRIES > 1) {
+            const unsigned long long y = __shfl_sync(0xffffffffu, e[ENTRIES - 1], i & 31);
+            if (i >= 32) x = y;
+        }
+        return x;
+    }
+};
+
+struct LogprobsParams {
+    const void* logits;
+    long long ld;
+    const int64_t* labels;
+    float *label_logprob, *entropy, *top_logprob;
+    int64_t *label_rank, *top_index;
+    int rows, classes, top;
+};
+
+__device__ __forceinline__ void lp_write(const LogprobsParams& p, long long row, int64_t label, float mine, const Part& all, unsigned long long before) {
+    const bool have = label >= 0 && label < p.classes, nothing = all.m == -INFINITY && all.s == 0.f;   // a row of -inf alone has no distribution
+    const float ls = logf(all.s);
+    if (p.label_logprob) p.label_logprob[row] = have ? (nothing ? -INFINITY : (mine - all.m) - ls) : label < 0 ? 0.f : __int_as_float(0x7fc00000);
+    if (p.label_rank) p.label_rank[row] = have ? (int64_t)before : -1;
+    if (p.entropy) p.entropy[row] = nothing ? 0.f : ls - all.w / all.s * LP_LN2;
+}
+__device__ __forceinline__ void lp_write_top(const LogprobsParams& p, long long row, int i, unsigned long long entry, const Part& all) {
+    const bool nothing = all.m == -INFINITY && all.s == 0.f;
+    p.top_logprob[row * p.top + i] = nothing ? -INFINITY : (key_value((uint32_t)(entry >> 32)) - all.m) - logf(all.s);
+    p.top_index[row * p.top + i] = (int64_t)(uint32_t)~(uint32_t)entry;
+}
+
+// A warp's share of a row: batches `part`, part + parts, ...  floor_s: a key that the row's k-th best is known to reach.
+template <typename T, int ENTRIES>
+__device__ __forceinline__ void lp_scan(const LogprobsParams& p, const T* row, int64_t label64, float& mine, int part, int parts, unsigned long long* queue,
+                                        uint32_t* floor_s, Part& all, unsigned& before, Best<ENTRIES>& best) {
+    constexpr int N = Vec<T>::N, VECS = 4, BATCH = 32 * VECS * N;
+    const int lane = threadIdx.x & 31, n = p.classes;
+    // vectors are counted from the 16-byte boundary at or below the row's first element, which is element `shift` there
+    const int shift = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+    const int step = parts * BATCH;
+    int first = part * BATCH - shift + lane * N;       // this lane's first element of the batch
+    Vec<T> v[VECS], ahead[VECS];
+#pragma unroll
+    for (int i = 0; i < VECS; i++) ahead[i].load(row, first + i * 32 * N, n);
+
+    const bool have = label64 >= 0 && label64 < n;
+    const int label = have ? (int)label64 : -1;
+    mine = have ? to_f32(row[label]) : 0.f;
+    // classes before the label: those at least as large as it in front of it, those larger behind it
     const uint32_t mykey = order_key(mine);
-    float s = 0.f, w = 0.f;
-    unsigned long long before = 0;
-    for (int j = threadIdx.x; j < classes; j += 256) {
-        const float v = to_f32(x[j]), d = v - m, e = expf(d);
-        const uint32_t key = order_key(v);
-        s += e;
-        w += fmaxf(d, -3e38f) * e;
-        before += key > mykey || (key == mykey && j < label);
-    }
-    s = block_reduce(s, add, fs);
-    w = block_reduce(w, add, fs);
-    before = block_reduce(before, [](unsigned long long a, unsigned long long b) { return a + b; }, us);
-    const float ls = logf(s);
-    unsigned long long best = 0;
-    for (int j = threadIdx.x; j < classes; j += 256) best = maxu(best, ((unsigned long long)order_key(to_f32(x[j])) << 32) | (uint32_t)~j);
-    best = block_reduce(best, maxu, us);
-    const bool nothing = (uint32_t)(best >> 32) == order_key(-INFINITY);   // a row of -inf alone has no distribution
-    if (threadIdx.x == 0) {
-        if (labels) {
-            if (label_logprob) label_logprob[row] = have ? (nothing ? -INFINITY : (mine - m) - ls) : label < 0 ? 0.f : __int_as_float(0x7fc00000);
-            if (label_rank) label_rank[row] = have ? (int64_t)before : -1;
+    const float thr_front = pass_from(mykey), thr_behind = pass_above(mykey);
+    const bool all_front = mine == -INFINITY, none_behind = mine != mine;   // (thresholds that would pass what is outside the row, or a NaN)
+
+    all = Part{-INFINITY, 0.f, 0.f};
+    before = 0;
+    if (have && all_front && part == 0 && lane == 0) before = label;
+#pragma unroll
+    for (int h = 0; h < ENTRIES; h++) best.e[h] = 0;
+    float thr = __int_as_float(0x7fc00000);            // passed by v where not (v <= thr)
+    bool fresh = true;                                 // the list has not been filled yet
+    const int batches = (int)(((long long)n + shift + BATCH - 1) / BATCH);
+    for (int b = part; b < batches; b += parts) {
+#pragma unroll
+        for (int i = 0; i < VECS; i++) v[i] = ahead[i];
+        if (b + parts < batches)
+#pragma unroll
+            for (int i = 0; i < VECS; i++) ahead[i].load(row, first + step + i * 32 * N, n);
+
+        float half[2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            half[h] = v[h * 2].value(0);
+#pragma unroll
+            for (int i = 0; i < 2 * N; i++) half[h] = ENTRIES ? max_nan(half[h], v[h * 2 + i / N].value(i % N)) : fmaxf(half[h], v[h * 2 + i / N].value(i % N));
         }
-        if (entropy) entropy[row] = nothing ? 0.f : ls - w / s;
-    }
-    for (int t = 0; t < top; t++) {
-        if (threadIdx.x == 0) {
-            const uint32_t key = (uint32_t)(best >> 32);
-            const float v = key == 0xffffffffu ? __int_as_float(0x7fc00000) : key_value(key);
-            if (top_logprob) top_logprob[row * top + t] = nothing ? -INFINITY : (v - m) - ls;
-            if (top_index) top_index[row * top + t] = (int64_t)(uint32_t)~(uint32_t)best;
+        const float top = max_nan(half[0], half[1]);
+        const float to = fmaxf(all.m, top);            // (a NaN is passed over: it makes S one)
+        if (to > all.m) all.raise(to);
+        const float base = all.m == -INFINITY ? 0.f : all.m;
+        float s[2] = {0.f, 0.f}, w[2] = {0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < VECS; i++)
+#pragma unroll
+            for (int e = 0; e < N; e++) {
+                const float t = max_nan((v[i].value(e) - base) * LP_LOG2E, LP_FLOOR), x = exp2_fast(t);
+                s[e & 1] += x;
+                w[e & 1] = fmaf(t, x, w[e & 1]);
+            }
+        all.s += s[0] + s[1];
+        all.w += w[0] + w[1];
+
+        if (have) {
+#pragma unroll
+            for (int i = 0; i < VECS; i++) {
+                const int at = first + i * 32 * N;
+                const bool front = at + N <= label, behind = at > label;
+                const float thr_rank = front ? thr_front : thr_behind;
+                unsigned c = 0;
+#pragma unroll
+                for (int e = 0; e < N; e++) c += !(v[i].value(e) <= thr_rank);
+                if (!front && !behind) {               // the label's own vector
+                    c = 0;
+#pragma unroll
+                    for (int e = 0; e < N; e++) {
+                        const bool inside = at + e >= 0 && at + e < n;
+                        if (inside && at + e < label && !all_front) c += !(v[i].value(e) <= thr_front);
+                        if (inside && at + e > label && !none_behind) c += !(v[i].value(e) <= thr_behind);
+                    }
+                } else if (front ? all_front : none_behind) c = 0;
+                before += c;
+            }
         }
-        unsigned long long next = 0;
-        for (int j = threadIdx.x; j < classes; j += 256) {
-            const unsigned long long k = ((unsigned long long)order_key(to_f32(x[j])) << 32) | (uint32_t)~j;
-            if (k < best) next = maxu(next, k);
+
+        if (ENTRIES) {
+            if (parts > 1) {
+                const uint32_t f = *reinterpret_cast<volatile uint32_t*>(floor_s);
+                if (f > 0x007fffffu) {                 // (above -inf) the k-th best of another warp: what equals it may still come before it
+                    const float t = pass_from(f);
+                    if (!(t <= thr)) thr = t;
+                }
+            }
+            uint32_t hot = __ballot_sync(0xffffffffu, !(top <= thr));
+            if (hot) {
+                if (fresh || __popc(hot) > 8) {
+                    // the top-th largest of the 64 half-lane maxima: as many classes are that large
+                    uint32_t a = order_key(half[0]), c = order_key(half[1]), kth = 0;
+                    for (int k = 0; k < p.top; k++) {
+                        const uint32_t mx = max(a, c);
+                        kth = __reduce_max_sync(0xffffffffu, mx);
+                        const int who = __ffs(__ballot_sync(0xffffffffu, mx == kth)) - 1;
+                        if (lane == who) { if (a >= c) a = 0; else c = 0; }
+                    }
+                    if (kth > 0x007fffffu) {           // (-inf may stand for what is outside the row)
+                        const float t = pass_from(kth);
+                        if (!(t <= thr) || thr != thr) thr = t;
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < VECS; i++) {
+                    int count = 0;
+#pragma unroll
+                    for (int e = 0; e < N; e++) {
+                        const int at = first + i * 32 * N + e;
+                        const bool hit = !(v[i].value(e) <= thr) && at >= 0 && at < n;
+                        const uint32_t mask = __ballot_sync(0xffffffffu, hit);
+                        if (hit) queue[count + __popc(mask & ((1u << lane) - 1))] = (unsigned long long)order_key(v[i].value(e)) << 32 | (uint32_t)~at;
+                        count += __popc(mask);
+                    }
+                    if (count) {
+                        __syncwarp();
+                        unsigned long long last = best.at(p.top - 1);
+                        for (int q = 0; q < count; q++) {
+                            const unsigned long long x = queue[q];
+                            if (x > last) {
+                                best.insert(x);
+                                last = best.at(p.top - 1);
+                            }
+                        }
+                        __syncwarp();
+                        if (last) {
+                            fresh = false;
+                            const uint32_t key = (uint32_t)(last >> 32);
+                            const float t = pass_above(key);
+                            if (!(t <= thr) || thr != thr) thr = t;
+                            if (parts > 1 && lane == 0) atomicMax(floor_s, key);
+                        }
+                    }
+                }
+            }
         }
-        best = block_reduce(next, maxu, us);
+        first += step;
     }
+    // the lanes' parts
+#pragma unroll
+    for (int d = 16; d; d >>= 1) {
+        Part o;
+        o.m = __shfl_xor_sync(0xffffffffu, all.m, d);
+        o.s = __shfl_xor_sync(0xffffffffu, all.s, d);
+        o.w = __shfl_xor_sync(0xffffffffu, all.w, d);
+        all.join(o);
+    }
+    before = __reduce_add_sync(0xffffffffu, before);
+}
+
+// a warp per row
+template <typename T, int ENTRIES>
+__global__ void __launch_bounds__(LP_WARPS * 32) logprobs_warp_kernel(const LogprobsParams p) {
+    __shared__ unsigned long long queue[ENTRIES ? LP_WARPS : 1][32 * Vec<T>::N];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const long long row = (long long)blockIdx.x * LP_WARPS + warp;
+    grid_dependency_wait();
+    if (row >= p.rows) return;
+    const int64_t label = p.labels ? p.labels[row] : -1;
+    float mine;
+    Part all;
+    unsigned before;
+    Best<ENTRIES> best;
+    lp_scan<T, ENTRIES>(p, static_cast<const T*>(p.logits) + row * p.ld, label, mine, 0, 1, queue[ENTRIES ? warp : 0], nullptr, all, before, best);
+    if (lane == 0) lp_write(p, row, label, mine, all, before);
+    if (ENTRIES)
+#pragma unroll
+        for (int h = 0; h < ENTRIES; h++)
+            if (h * 32 + lane < p.top) lp_write_top(p, row, h * 32 + lane, best.e[h], all);
+}
+
+// a cluster of CTAs (one, where rows are many) per row
+template <typename T, int ENTRIES>
+__global__ void __launch_bounds__(LP_WARPS * 32) logprobs_team_kernel(const LogprobsParams p, const int ctas) {
+    constexpr int LIST = ENTRIES ? ENTRIES * 32 : 1;
+    __shared__ unsigned long long queue[ENTRIES ? LP_WARPS : 1][32 * Vec<T>::N];
+    __shared__ unsigned long long lists[LP_WARPS][LIST], merged[LIST], gathered[LP_MAX_CLUSTER * LIST];
+    __shared__ Part parts[LP_WARPS], part_s;
+    __shared__ unsigned before_s[LP_WARPS], before_cta;
+    __shared__ uint32_t floor_s;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = blockIdx.x % ctas;
+    const long long row = blockIdx.x / ctas;
+    if (threadIdx.x == 0) floor_s = 0;
+    __syncthreads();
+    grid_dependency_wait();
+    const int64_t label = p.labels ? p.labels[row] : -1;
+    float mine;
+    Part all;
+    unsigned before;
+    Best<ENTRIES> best;
+    lp_scan<T, ENTRIES>(p, static_cast<const T*>(p.logits) + row * p.ld, label, mine, warp * ctas + rank, LP_WARPS * ctas, queue[ENTRIES ? warp : 0], &floor_s, all,
+                        before, best);
+    if (lane == 0) { parts[warp] = all; before_s[warp] = before; }
+    if (ENTRIES)
+#pragma unroll
+        for (int h = 0; h < ENTRIES; h++) lists[warp][h * 32 + lane] = h * 32 + lane < p.top ? best.e[h] : 0;
+    __syncthreads();
+    all = parts[0];
+    before = before_s[0];
+#pragma unroll
+    for (int i = 1; i < LP_WARPS; i++) { all.join(parts[i]); before += before_s[i]; }
+    // an entry's place: how many of the others come before it (no two are alike; 0 stands for none)
+    auto place = [&](const unsigned long long* entries, int stride, int count, unsigned long long x) {
+        int better = 0;
+        for (int i = 0; i < count; i++)
+            for (int k = 0; k < p.top; k++) better += entries[i * stride + k] > x;
+        return better;
+    };
+    if (ENTRIES) {
+        if (ctas > 1) {
+            for (int i = threadIdx.x; i < LIST; i += LP_WARPS * 32) merged[i] = 0;
+            __syncthreads();
+        }
+        for (int i = threadIdx.x; i < LP_WARPS * p.top; i += LP_WARPS * 32) {
+            const unsigned long long x = lists[i / p.top][i % p.top];
+            const int at = x ? place(&lists[0][0], LIST, LP_WARPS, x) : p.top;
+            if (at < p.top) {
+                if (ctas > 1) merged[at] = x;
+                else lp_write_top(p, row, at, x, all);
+            }
+        }
+    }
+    if (ctas == 1) {
+        if (threadIdx.x == 0) lp_write(p, row, label, mine, all, before);
+        return;
+    }
+    if (threadIdx.x == 0) { part_s = all; before_cta = before; }
+    auto cluster_sync = [] { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); };
+    __syncwarp();
+    cluster_sync();
+    if (rank == 0) {
+        auto there = [](const void* here, int r) {
+            uint32_t a;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(here)), "r"(r));
+            return a;
+        };
+        auto read = [](uint32_t a) {
+            uint32_t x;
+            asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(x) : "r"(a) : "memory");
+            return x;
+        };
+        if (ENTRIES)
+            for (int i = threadIdx.x; i < ctas * p.top; i += LP_WARPS * 32) {
+                unsigned long long x;
+                asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(x) : "r"(there(&merged[i % p.top], i / p.top)) : "memory");
+                gathered[i / p.top * LIST + i % p.top] = x;
+            }
+        Part o[LP_MAX_CLUSTER];
+        unsigned c[LP_MAX_CLUSTER];
+#pragma unroll
+        for (int r = 1; r < LP_MAX_CLUSTER; r++)
+            if (r < ctas) {
+                const uint32_t a = there(&part_s, r);
+                o[r] = Part{__uint_as_float(read(a)), __uint_as_float(read(a + 4)), __uint_as_float(read(a + 8))};
+                c[r] = read(there(&before_cta, r));
+            }
+#pragma unroll
+        for (int r = 1; r < LP_MAX_CLUSTER; r++)
+            if (r < ctas) { all.join(o[r]); before += c[r]; }
+        __syncthreads();
+        if (threadIdx.x == 0) lp_write(p, row, label, mine, all, before);
+        if (ENTRIES)
+            for (int i = threadIdx.x; i < ctas * p.top; i += LP_WARPS * 32) {
+                const unsigned long long x = gathered[i / p.top * LIST + i % p.top];
+                const int at = x ? place(gathered, LIST, ctas, x) : p.top;
+                if (at < p.top) lp_write_top(p, row, at, x, all);
+            }
+    }
+    __syncwarp();
+    cluster_sync();                                    // no CTA leaves while its part is being read
+}
+
+// Rows of one batch have a warp each, and so do those of up to 4096 classes where there are rows for every scheduler; others a
+// CTA, or as many CTAs (up to 8) as keep the SMs busy and find a batch for each of their warps.
+template <typename T, int ENTRIES>
+static int lp_launch(const LogprobsParams& p, cudaStream_t stream) {
+    if (p.classes <= 128 * Vec<T>::N || (p.classes <= 4096 && p.rows >= 4 * sm_count())) {
+        DABNN_CUDA_OK(launch_overlapped(logprobs_warp_kernel<T, ENTRIES>, dim3((unsigned)(((long long)p.rows + LP_WARPS - 1) / LP_WARPS)), dim3(LP_WARPS * 32), 0, stream, p));
+        return DABNN_OK;
+    }
+    int ctas = 1;
+    while (ctas < LP_MAX_CLUSTER && (long long)p.rows * ctas * 2 <= 2 * sm_count() && (long long)ctas * LP_WARPS * 128 * Vec<T>::N < p.classes) ctas *= 2;
+    DABNN_REQUIRE((long long)p.rows * ctas <= INT_MAX, DABNN_ERR_SHAPE, "logprobs: too many rows");
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(p.rows * ctas));
+    cfg.blockDim = dim3(LP_WARPS * 32);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ctas;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = g_overlap_launches ? 2 : 1;
+    DABNN_CUDA_OK(cudaLaunchKernelEx(&cfg, logprobs_team_kernel<T, ENTRIES>, p, ctas));
+    return DABNN_OK;
 }
 
 }  // namespace dabnn
@@ -101,6 +468,7 @@ extern "C" int dabnn_logprobs(const void* logits, int type, long long ld, const 
                               int64_t* label_rank, float* entropy, float* top_logprob, int64_t* top_index, int top, dabnn_stream_t s) {
     DABNN_REQUIRE(type >= DABNN_F32 && type <= DABNN_BF16, DABNN_ERR_ARG, "logprobs: unknown type");
     DABNN_REQUIRE(rows >= 0 && classes >= 1, DABNN_ERR_ARG, "logprobs: bad dims");
+    DABNN_REQUIRE(classes < INT_MAX / 2, DABNN_ERR_SHAPE, "logprobs: too many classes");
     DABNN_REQUIRE(top >= 0 && top <= DABNN_LOGPROBS_MAX_TOP && top <= classes, DABNN_ERR_ARG, "logprobs: top must be between 0 and the smaller of 64 and the classes");
     if (rows == 0) return DABNN_OK;
     DABNN_REQUIRE(labels || (!label_logprob && !label_rank), DABNN_ERR_ARG, "logprobs: a label's outputs without labels");
@@ -109,12 +477,12 @@ extern "C" int dabnn_logprobs(const void* logits, int type, long long ld, const 
     DABNN_REQUIRE(ld >= classes || rows == 1, DABNN_ERR_SHAPE, "logprobs: the row pitch is below the classes");
     DABNN_REQUIRE((reinterpret_cast<uintptr_t>(logits) & (type == DABNN_F32 ? 3 : 1)) == 0, DABNN_ERR_ARG, "logprobs: misaligned pointer");
     const cudaStream_t stream = static_cast<cudaStream_t>(s);
+    const LogprobsParams p{logits, ld, labels, label_logprob, entropy, top_logprob, label_rank, top_index, rows, classes, top};
     auto launch = [&](auto tag) {
         using T = decltype(tag);
-        logprobs_kernel<T><<<rows, 256, 0, stream>>>(static_cast<const T*>(logits), ld, labels, classes, label_logprob, label_rank, entropy, top_logprob, top_index, top);
+        return top == 0 ? lp_launch<T, 0>(p, stream) : top <= 32 ? lp_launch<T, 1>(p, stream) : lp_launch<T, 2>(p, stream);
     };
-    if (type == DABNN_F32) launch(float{});
-    else if (type == DABNN_F16) launch(__half{});
-    else launch(__nv_bfloat16{});
-    return check_launch("logprobs_kernel");
+    if (type == DABNN_F32) return launch(float{});
+    if (type == DABNN_F16) return launch(__half{});
+    return launch(__nv_bfloat16{});
 }
