@@ -5,12 +5,12 @@
 //
 // Classes are ordered by value, larger first, equal ones (the two zeros are) by index, a NaN before everything.
 //
-// One pass over a row, no lane waiting for another: a lane keeps its own m, S, W (rescaled when its m grows) and its own count
-// of classes before the label; a warp keeps its best classes in order, one to a lane.  A batch of a warp - 64 bytes of each
-// lane - is looked at for alternatives only if some lane's maximum passes the warp's threshold (its k-th best, or another
-// warp's of the row), which after a row's first batches is rare.  What it finds goes through a queue in shared memory and is
-// inserted one by one.  The first batch has no threshold yet: the k-th largest of the 64 half-lane maxima is one, since there are
-// then at least k classes that reach it.
+// One pass over a row: a lane keeps its own m, S, W (rescaled when its m grows) and its own count of classes before the label;
+// a warp keeps its best classes in order, one to a lane.  A batch of a warp - 64 bytes of each lane - is looked at for
+// alternatives only if some lane's maximum passes a threshold: the warp's k-th best, or that of the row's eight warps, which
+// is found after 1, 2, 4, ... rounds of batches.  What passes goes through a queue in shared memory and is inserted one by one.
+// The first batch has no threshold yet: the k-th largest of the 64 half-lane maxima is one, since there are then at least k
+// classes that reach it.
 //
 // A row is scored by one warp, or by a CTA of eight, or by a cluster of such CTAs where rows are few: the warps take the row's
 // batches in turn and their parts are joined at the end, lists of best classes by counting, for each entry, the better ones.
@@ -57,6 +57,26 @@ __device__ __forceinline__ float exp2_fast(float x) {   // ex2.approx: off by 2^
     return r;
 }
 
+// two fp32 operations in an instruction
+__device__ __forceinline__ float2 two_add(float2 a, float2 b) {
+    float2 r;
+    asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ float2 two_mul(float2 a, float2 b) {
+    float2 r;
+    asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ float2 two_fma(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return r;
+}
+
 // Part of a row: its maximum, and S and W relative to it, W in units of ln 2 (the argument that ex2 wants anyway)
 struct Part {
     float m, s, w;
@@ -85,6 +105,7 @@ struct Vec {                                           // 16 bytes of a row
         else if constexpr (std::is_same_v<T, __nv_bfloat16>) return __uint_as_float(i % 2 ? w & 0xffff0000u : w << 16);
         else return __half2float(__ushort_as_half((unsigned short)(i % 2 ? w >> 16 : w)));
     }
+    __device__ __forceinline__ uint32_t word(int i) const { return i == 0 ? raw.x : i == 1 ? raw.y : i == 2 ? raw.z : raw.w; }
     // values at [first, first + N) of a row of n, -inf outside it; `row` + first is on a 16-byte boundary
     __device__ __forceinline__ void load(const T* row, int first, int n) {
         if (first >= 0 && first + N <= n) {
@@ -158,10 +179,81 @@ __device__ __forceinline__ void lp_write_top(const LogprobsParams& p, long long 
     p.top_index[row * p.top + i] = (int64_t)(uint32_t)~(uint32_t)entry;
 }
 
-// A warp's share of a row: batches `part`, part + parts, ...  floor_s: a key that the row's k-th best is known to reach.
-template <typename T, int ENTRIES>
+// Two 16-bit values at a time: the larger (a NaN wins), and how many pass a threshold, not (v <= t), as two small floats
+template <typename T> struct Pair16;
+template <> struct Pair16<__half> {
+    static __device__ __forceinline__ uint32_t max(uint32_t a, uint32_t b) { uint32_t r; asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r; }
+    static __device__ __forceinline__ uint32_t count(uint32_t v, uint32_t t, uint32_t sum) {
+        uint32_t r;
+        asm("{\n\t.reg .b32 c;\n\tset.gtu.f16x2.f16x2 c, %1, %2;\n\tadd.f16x2 %0, c, %3;\n\t}" : "=r"(r) : "r"(v), "r"(t), "r"(sum));
+        return r;
+    }
+    static __device__ __forceinline__ uint32_t bits(float t) { return __half_as_ushort(__float2half_rd(t)); }
+    static __device__ __forceinline__ float value(uint32_t b) { return __half2float(__ushort_as_half((unsigned short)b)); }
+};
+template <> struct Pair16<__nv_bfloat16> {
+    static __device__ __forceinline__ uint32_t max(uint32_t a, uint32_t b) { uint32_t r; asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r; }
+    static __device__ __forceinline__ uint32_t count(uint32_t v, uint32_t t, uint32_t sum) {
+        uint32_t r;
+        asm("{\n\t.reg .b32 c;\n\tset.gtu.bf16x2.bf16x2 c, %1, %2;\n\tadd.bf16x2 %0, c, %3;\n\t}" : "=r"(r) : "r"(v), "r"(t), "r"(sum));
+        return r;
+    }
+    static __device__ __forceinline__ uint32_t bits(float t) { return __bfloat16_as_ushort(__float2bfloat16_rd(t)); }
+    static __device__ __forceinline__ float value(uint32_t b) { return __uint_as_float(b << 16); }
+};
+
+// the largest of two vectors (a NaN wins)
+template <typename T>
+__device__ __forceinline__ float vec_max(const Vec<T>& a, const Vec<T>& b) {
+    if constexpr (sizeof(T) == 4) {
+        float m = max_nan(a.value(0), b.value(0));
+#pragma unroll
+        for (int i = 1; i < 4; i++) m = max_nan(m, max_nan(a.value(i), b.value(i)));
+        return m;
+    } else {
+        uint32_t m = Pair16<T>::max(a.raw.x, b.raw.x);
+#pragma unroll
+        for (int i = 1; i < 4; i++) m = Pair16<T>::max(m, Pair16<T>::max(a.word(i), b.word(i)));
+        return max_nan(Pair16<T>::value(m & 0xffffu), Pair16<T>::value(m >> 16));
+    }
+}
+// how many of a vector's values pass: not (v <= t)
+template <typename T>
+__device__ __forceinline__ unsigned vec_count(const Vec<T>& v, float t) {
+    if constexpr (sizeof(T) == 4) {
+        unsigned c = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) c += !(v.value(i) <= t);
+        return c;
+    } else {   // (t rounded down to the type passes the same values)
+        const uint32_t b = Pair16<T>::bits(t), tt = b | b << 16;
+        uint32_t c = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) c = Pair16<T>::count(v.word(i), tt, c);
+        return (unsigned)(Pair16<T>::value(c & 0xffffu) + Pair16<T>::value(c >> 16));
+    }
+}
+
+// how many entries of a list in order come before x (zeros, which stand for none, are at the end)
+__device__ __forceinline__ int entries_before(const unsigned long long* list, int n, unsigned long long x) {
+    int at = 0;
+#pragma unroll
+    for (int s = DABNN_LOGPROBS_MAX_TOP; s; s >>= 1)
+        if (at + s <= n && list[at + s - 1] > x) at += s;
+    return at;
+}
+
+// What the warps of a CTA share about their row's best classes
+template <int ENTRIES>
+struct Shared {
+    unsigned long long lists[LP_WARPS][ENTRIES ? ENTRIES * 32 : 1];   // each warp's, in order
+    unsigned long long floor;                          // an entry that the row's k-th best is known to be or to come before
+};
+
+// A warp's share of a row: batches `part`, part + parts, ...
+template <typename T, int ENTRIES, bool TEAM>
 __device__ __forceinline__ void lp_scan(const LogprobsParams& p, const T* row, int64_t label64, float& mine, int part, int parts, unsigned long long* queue,
-                                        uint32_t* floor_s, Part& all, unsigned& before, Best<ENTRIES>& best) {
+                                        Shared<ENTRIES>* shared, Part& all, unsigned& before, Best<ENTRIES>& best) {
     constexpr int N = Vec<T>::N, VECS = 4, BATCH = 32 * VECS * N;
     const int lane = threadIdx.x & 31, n = p.classes;
     // vectors are counted from the 16-byte boundary at or below the row's first element, which is element `shift` there
@@ -185,72 +277,57 @@ __device__ __forceinline__ void lp_scan(const LogprobsParams& p, const T* row, i
     if (have && all_front && part == 0 && lane == 0) before = label;
 #pragma unroll
     for (int h = 0; h < ENTRIES; h++) best.e[h] = 0;
-    float thr = __int_as_float(0x7fc00000);            // passed by v where not (v <= thr)
+    float thr = __int_as_float(0x7fc00000);            // an alternative is what passes: not (v <= thr)
     bool fresh = true;                                 // the list has not been filled yet
-    const int batches = (int)(((long long)n + shift + BATCH - 1) / BATCH);
-    for (int b = part; b < batches; b += parts) {
+    const int batches = (int)(((long long)n + shift + BATCH - 1) / BATCH), rounds = (batches + parts - 1) / parts;
+    for (int round = 0, b = part; round < rounds; round++, b += parts) {
 #pragma unroll
         for (int i = 0; i < VECS; i++) v[i] = ahead[i];
         if (b + parts < batches)
 #pragma unroll
             for (int i = 0; i < VECS; i++) ahead[i].load(row, first + step + i * 32 * N, n);
+        if (b < batches) {
+            const float half[2] = {vec_max(v[0], v[1]), vec_max(v[2], v[3])};
+            const float top = max_nan(half[0], half[1]);
+            const float to = fmaxf(all.m, top);        // (a NaN is passed over: it makes S one)
+            if (to > all.m) all.raise(to);
+            const float base = all.m == -INFINITY ? 0.f : all.m;
+            float2 s = make_float2(0.f, 0.f), w = s;
+#pragma unroll
+            for (int i = 0; i < VECS; i++)
+#pragma unroll
+                for (int e = 0; e < N; e += 2) {
+                    float2 t = two_mul(two_add(make_float2(v[i].value(e), v[i].value(e + 1)), make_float2(-base, -base)), make_float2(LP_LOG2E, LP_LOG2E));
+                    t = make_float2(max_nan(t.x, LP_FLOOR), max_nan(t.y, LP_FLOOR));
+                    const float2 x = make_float2(exp2_fast(t.x), exp2_fast(t.y));
+                    s = two_add(s, x);
+                    w = two_fma(t, x, w);
+                }
+            all.s += s.x + s.y;
+            all.w += w.x + w.y;
 
-        float half[2];
+            if (have) {
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            half[h] = v[h * 2].value(0);
+                for (int i = 0; i < VECS; i++) {
+                    const int at = first + i * 32 * N;
+                    const bool front = at + N <= label;
+                    unsigned c = vec_count(v[i], front ? thr_front : thr_behind);
+                    if (front ? all_front : none_behind) c = 0;
+                    if (at <= label && !front) {       // the label's own vector
+                        c = 0;
 #pragma unroll
-            for (int i = 0; i < 2 * N; i++) half[h] = ENTRIES ? max_nan(half[h], v[h * 2 + i / N].value(i % N)) : fmaxf(half[h], v[h * 2 + i / N].value(i % N));
-        }
-        const float top = max_nan(half[0], half[1]);
-        const float to = fmaxf(all.m, top);            // (a NaN is passed over: it makes S one)
-        if (to > all.m) all.raise(to);
-        const float base = all.m == -INFINITY ? 0.f : all.m;
-        float s[2] = {0.f, 0.f}, w[2] = {0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < VECS; i++)
-#pragma unroll
-            for (int e = 0; e < N; e++) {
-                const float t = max_nan((v[i].value(e) - base) * LP_LOG2E, LP_FLOOR), x = exp2_fast(t);
-                s[e & 1] += x;
-                w[e & 1] = fmaf(t, x, w[e & 1]);
-            }
-        all.s += s[0] + s[1];
-        all.w += w[0] + w[1];
-
-        if (have) {
-#pragma unroll
-            for (int i = 0; i < VECS; i++) {
-                const int at = first + i * 32 * N;
-                const bool front = at + N <= label, behind = at > label;
-                const float thr_rank = front ? thr_front : thr_behind;
-                unsigned c = 0;
-#pragma unroll
-                for (int e = 0; e < N; e++) c += !(v[i].value(e) <= thr_rank);
-                if (!front && !behind) {               // the label's own vector
-                    c = 0;
-#pragma unroll
-                    for (int e = 0; e < N; e++) {
-                        const bool inside = at + e >= 0 && at + e < n;
-                        if (inside && at + e < label && !all_front) c += !(v[i].value(e) <= thr_front);
-                        if (inside && at + e > label && !none_behind) c += !(v[i].value(e) <= thr_behind);
+                        for (int e = 0; e < N; e++) {
+                            const bool inside = at + e >= 0 && at + e < n;
+                            if (inside && at + e < label && !all_front) c += !(v[i].value(e) <= thr_front);
+                            if (inside && at + e > label && !none_behind) c += !(v[i].value(e) <= thr_behind);
+                        }
                     }
-                } else if (front ? all_front : none_behind) c = 0;
-                before += c;
-            }
-        }
-
-        if (ENTRIES) {
-            if (parts > 1) {
-                const uint32_t f = *reinterpret_cast<volatile uint32_t*>(floor_s);
-                if (f > 0x007fffffu) {                 // (above -inf) the k-th best of another warp: what equals it may still come before it
-                    const float t = pass_from(f);
-                    if (!(t <= thr)) thr = t;
+                    before += c;
                 }
             }
-            uint32_t hot = __ballot_sync(0xffffffffu, !(top <= thr));
-            if (hot) {
-                if (fresh || __popc(hot) > 8) {
+
+            if (ENTRIES && __any_sync(0xffffffffu, !(top <= thr))) {
+                if (fresh || __popc(__ballot_sync(0xffffffffu, !(top <= thr))) > 8) {
                     // the top-th largest of the 64 half-lane maxima: as many classes are that large
                     uint32_t a = order_key(half[0]), c = order_key(half[1]), kth = 0;
                     for (int k = 0; k < p.top; k++) {
@@ -261,43 +338,66 @@ __device__ __forceinline__ void lp_scan(const LogprobsParams& p, const T* row, i
                     }
                     if (kth > 0x007fffffu) {           // (-inf may stand for what is outside the row)
                         const float t = pass_from(kth);
-                        if (!(t <= thr) || thr != thr) thr = t;
+                        if (!(t <= thr)) thr = t;
                     }
                 }
-#pragma unroll
+                unsigned long long last = best.at(p.top - 1);
+#pragma unroll 1
                 for (int i = 0; i < VECS; i++) {
+                    Vec<T> u = v[0];
+#pragma unroll
+                    for (int k = 1; k < VECS; k++)
+                        if (i == k) u = v[k];
+                    if (!__any_sync(0xffffffffu, !(vec_max(u, u) <= thr))) continue;
                     int count = 0;
 #pragma unroll
                     for (int e = 0; e < N; e++) {
                         const int at = first + i * 32 * N + e;
-                        const bool hit = !(v[i].value(e) <= thr) && at >= 0 && at < n;
+                        const bool hit = !(u.value(e) <= thr) && at >= 0 && at < n;
                         const uint32_t mask = __ballot_sync(0xffffffffu, hit);
-                        if (hit) queue[count + __popc(mask & ((1u << lane) - 1))] = (unsigned long long)order_key(v[i].value(e)) << 32 | (uint32_t)~at;
+                        if (hit) queue[count + __popc(mask & ((1u << lane) - 1))] = (unsigned long long)order_key(u.value(e)) << 32 | (uint32_t)~at;
                         count += __popc(mask);
                     }
-                    if (count) {
-                        __syncwarp();
-                        unsigned long long last = best.at(p.top - 1);
-                        for (int q = 0; q < count; q++) {
-                            const unsigned long long x = queue[q];
-                            if (x > last) {
-                                best.insert(x);
-                                last = best.at(p.top - 1);
-                            }
+                    __syncwarp();
+#pragma unroll 1
+                    for (int q = 0; q < count; q++) {
+                        const unsigned long long x = queue[q];
+                        if (x > last) {
+                            best.insert(x);
+                            last = best.at(p.top - 1);
                         }
-                        __syncwarp();
-                        if (last) {
-                            fresh = false;
-                            const uint32_t key = (uint32_t)(last >> 32);
-                            const float t = pass_above(key);
-                            if (!(t <= thr) || thr != thr) thr = t;
-                            if (parts > 1 && lane == 0) atomicMax(floor_s, key);
-                        }
+                    }
+                    __syncwarp();
+                    if (last) {                        // in a warp's own order what equals it comes after it
+                        fresh = false;
+                        const float t = pass_above((uint32_t)(last >> 32));
+                        if (!(t <= thr)) thr = t;
                     }
                 }
             }
         }
         first += step;
+        // the k-th best of all eight warps so far, after 1, 2, 4, ... rounds
+        if (TEAM && ENTRIES && round + 1 < rounds && (round & (round + 1)) == 0) {
+#pragma unroll
+            for (int h = 0; h < ENTRIES; h++) shared->lists[threadIdx.x >> 5][h * 32 + lane] = best.e[h];
+            __syncthreads();
+            for (int i = threadIdx.x; i < LP_WARPS * p.top; i += LP_WARPS * 32) {
+                const unsigned long long x = shared->lists[i / p.top][i % p.top];
+                int at = 0;
+                if (x)
+                    for (int k = 0; k < LP_WARPS; k++) at += entries_before(shared->lists[k], p.top, x);
+                if (x && at == p.top - 1) shared->floor = x;
+            }
+            __syncthreads();
+            const unsigned long long f = shared->floor;
+            const uint32_t key = (uint32_t)(f >> 32);
+            if (key > 0x007fffffu) {                   // its equals pass only while they may come before it
+                const bool later = (b + parts) * BATCH - shift > (int)~(uint32_t)f;
+                const float t = later ? pass_above(key) : pass_from(key);
+                if (!(t <= thr)) thr = t;
+            }
+        }
     }
     // the lanes' parts
 #pragma unroll
@@ -313,7 +413,7 @@ __device__ __forceinline__ void lp_scan(const LogprobsParams& p, const T* row, i
 
 // a warp per row
 template <typename T, int ENTRIES>
-__global__ void __launch_bounds__(LP_WARPS * 32) logprobs_warp_kernel(const LogprobsParams p) {
+__global__ void __launch_bounds__(LP_WARPS * 32, 3) logprobs_warp_kernel(const LogprobsParams p) {
     __shared__ unsigned long long queue[ENTRIES ? LP_WARPS : 1][32 * Vec<T>::N];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const long long row = (long long)blockIdx.x * LP_WARPS + warp;
@@ -324,7 +424,7 @@ __global__ void __launch_bounds__(LP_WARPS * 32) logprobs_warp_kernel(const Logp
     Part all;
     unsigned before;
     Best<ENTRIES> best;
-    lp_scan<T, ENTRIES>(p, static_cast<const T*>(p.logits) + row * p.ld, label, mine, 0, 1, queue[ENTRIES ? warp : 0], nullptr, all, before, best);
+    lp_scan<T, ENTRIES, false>(p, static_cast<const T*>(p.logits) + row * p.ld, label, mine, 0, 1, queue[ENTRIES ? warp : 0], nullptr, all, before, best);
     if (lane == 0) lp_write(p, row, label, mine, all, before);
     if (ENTRIES)
 #pragma unroll
@@ -334,16 +434,16 @@ __global__ void __launch_bounds__(LP_WARPS * 32) logprobs_warp_kernel(const Logp
 
 // a cluster of CTAs (one, where rows are many) per row
 template <typename T, int ENTRIES>
-__global__ void __launch_bounds__(LP_WARPS * 32) logprobs_team_kernel(const LogprobsParams p, const int ctas) {
+__global__ void __launch_bounds__(LP_WARPS * 32, 3) logprobs_team_kernel(const LogprobsParams p, const int ctas) {
     constexpr int LIST = ENTRIES ? ENTRIES * 32 : 1;
     __shared__ unsigned long long queue[ENTRIES ? LP_WARPS : 1][32 * Vec<T>::N];
-    __shared__ unsigned long long lists[LP_WARPS][LIST], merged[LIST], gathered[LP_MAX_CLUSTER * LIST];
+    __shared__ Shared<ENTRIES> shared;
+    __shared__ unsigned long long merged[LIST], gathered[LP_MAX_CLUSTER * LIST];
     __shared__ Part parts[LP_WARPS], part_s;
     __shared__ unsigned before_s[LP_WARPS], before_cta;
-    __shared__ uint32_t floor_s;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = blockIdx.x % ctas;
     const long long row = blockIdx.x / ctas;
-    if (threadIdx.x == 0) floor_s = 0;
+    if (threadIdx.x == 0) shared.floor = 0;
     __syncthreads();
     grid_dependency_wait();
     const int64_t label = p.labels ? p.labels[row] : -1;
@@ -351,22 +451,21 @@ __global__ void __launch_bounds__(LP_WARPS * 32) logprobs_team_kernel(const Logp
     Part all;
     unsigned before;
     Best<ENTRIES> best;
-    lp_scan<T, ENTRIES>(p, static_cast<const T*>(p.logits) + row * p.ld, label, mine, warp * ctas + rank, LP_WARPS * ctas, queue[ENTRIES ? warp : 0], &floor_s, all,
-                        before, best);
+    lp_scan<T, ENTRIES, true>(p, static_cast<const T*>(p.logits) + row * p.ld, label, mine, warp * ctas + rank, LP_WARPS * ctas, queue[ENTRIES ? warp : 0], &shared, all,
+                              before, best);
     if (lane == 0) { parts[warp] = all; before_s[warp] = before; }
     if (ENTRIES)
 #pragma unroll
-        for (int h = 0; h < ENTRIES; h++) lists[warp][h * 32 + lane] = h * 32 + lane < p.top ? best.e[h] : 0;
+        for (int h = 0; h < ENTRIES; h++) shared.lists[warp][h * 32 + lane] = best.e[h];
     __syncthreads();
     all = parts[0];
     before = before_s[0];
 #pragma unroll
     for (int i = 1; i < LP_WARPS; i++) { all.join(parts[i]); before += before_s[i]; }
     // an entry's place: how many of the others come before it (no two are alike; 0 stands for none)
-    auto place = [&](const unsigned long long* entries, int stride, int count, unsigned long long x) {
+    auto place = [&](const unsigned long long* entries, int count, unsigned long long x) {
         int better = 0;
-        for (int i = 0; i < count; i++)
-            for (int k = 0; k < p.top; k++) better += entries[i * stride + k] > x;
+        for (int i = 0; i < count; i++) better += entries_before(entries + i * LIST, p.top, x);
         return better;
     };
     if (ENTRIES) {
@@ -375,8 +474,8 @@ __global__ void __launch_bounds__(LP_WARPS * 32) logprobs_team_kernel(const Logp
             __syncthreads();
         }
         for (int i = threadIdx.x; i < LP_WARPS * p.top; i += LP_WARPS * 32) {
-            const unsigned long long x = lists[i / p.top][i % p.top];
-            const int at = x ? place(&lists[0][0], LIST, LP_WARPS, x) : p.top;
+            const unsigned long long x = shared.lists[i / p.top][i % p.top];
+            const int at = x ? place(&shared.lists[0][0], LP_WARPS, x) : p.top;
             if (at < p.top) {
                 if (ctas > 1) merged[at] = x;
                 else lp_write_top(p, row, at, x, all);
@@ -425,7 +524,7 @@ __global__ void __launch_bounds__(LP_WARPS * 32) logprobs_team_kernel(const Logp
         if (ENTRIES)
             for (int i = threadIdx.x; i < ctas * p.top; i += LP_WARPS * 32) {
                 const unsigned long long x = gathered[i / p.top * LIST + i % p.top];
-                const int at = x ? place(gathered, LIST, ctas, x) : p.top;
+                const int at = x ? place(gathered, ctas, x) : p.top;
                 if (at < p.top) lp_write_top(p, row, at, x, all);
             }
     }
