@@ -5,12 +5,13 @@
 //
 // Classes are ordered by value, larger first, equal ones (the two zeros are) by index, a NaN before everything.
 //
-// One pass over a row: a lane keeps its own m, S, W (rescaled when its m grows) and its own count of classes before the label;
-// a warp keeps its best classes in order, one to a lane.  A batch of a warp - 64 bytes of each lane - is looked at for
-// alternatives only if some lane's maximum passes a threshold: the warp's k-th best, or that of the row's eight warps, which
-// is found after 1, 2, 4, ... rounds of batches.  What passes goes through a queue in shared memory and is inserted one by one.
-// The first batch has no threshold yet: the k-th largest of the 64 half-lane maxima is one, since there are then at least k
-// classes that reach it.
+// One pass over a row, no warp waiting for another: a lane keeps its own m, S, W (rescaled when its m grows) and its own count
+// of classes before the label; a warp keeps its best classes in order, one to a lane.  A batch of a warp - 64 bytes of each
+// lane - is looked at for alternatives only if some lane's maximum passes a threshold: the warp's k-th best, or the least of
+// the eight warps' ceil(k / 8)-th bests (k classes of the row reach that).  The lanes that pass leave their 64 bytes in shared
+// memory, where the warp looks at the values of one lane (two of fp32) at a time, inserting what belongs among the best.  The
+// first batch has no threshold yet: the k-th largest of the 64 half-lane maxima is one, since there are then at least k classes
+// that reach it.
 //
 // A row is scored by one warp, or by a CTA of eight, or by a cluster of such CTAs where rows are few: the warps take the row's
 // batches in turn and their parts are joined at the end, lists of best classes by counting, for each entry, the better ones.
@@ -217,22 +218,27 @@ __device__ __forceinline__ float vec_max(const Vec<T>& a, const Vec<T>& b) {
         return max_nan(Pair16<T>::value(m & 0xffffu), Pair16<T>::value(m >> 16));
     }
 }
-// how many of a vector's values pass: not (v <= t)
+// How many values of a vector pass, not (v <= t), added to a running count: whole numbers in one float, or in two small ones
+// (t rounded down to a 16-bit type passes the same values of it)
 template <typename T>
-__device__ __forceinline__ unsigned vec_count(const Vec<T>& v, float t) {
-    if constexpr (sizeof(T) == 4) {
-        unsigned c = 0;
-#pragma unroll
-        for (int i = 0; i < 4; i++) c += !(v.value(i) <= t);
-        return c;
-    } else {   // (t rounded down to the type passes the same values)
-        const uint32_t b = Pair16<T>::bits(t), tt = b | b << 16;
-        uint32_t c = 0;
-#pragma unroll
-        for (int i = 0; i < 4; i++) c = Pair16<T>::count(v.word(i), tt, c);
-        return (unsigned)(Pair16<T>::value(c & 0xffffu) + Pair16<T>::value(c >> 16));
+struct Count {
+    using Threshold = std::conditional_t<sizeof(T) == 4, float, uint32_t>;
+    static __device__ __forceinline__ Threshold threshold(float t) {
+        if constexpr (sizeof(T) == 4) return t;
+        else return Pair16<T>::bits(t) * 0x10001u;
     }
-}
+    Threshold sum = 0;
+    __device__ __forceinline__ void add(const Vec<T>& v, Threshold t) {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if constexpr (sizeof(T) == 4) sum += v.value(i) <= t ? 0.f : 1.f;
+            else sum = Pair16<T>::count(v.word(i), t, sum);
+    }
+    __device__ __forceinline__ int total() const {
+        if constexpr (sizeof(T) == 4) return (int)sum;
+        else return (int)(Pair16<T>::value(sum & 0xffffu) + Pair16<T>::value(sum >> 16));
+    }
+};
 
 // how many entries of a list in order come before x (zeros, which stand for none, are at the end)
 __device__ __forceinline__ int entries_before(const unsigned long long* list, int n, unsigned long long x) {
@@ -246,13 +252,18 @@ __device__ __forceinline__ int entries_before(const unsigned long long* list, in
 // What the warps of a CTA share about their row's best classes
 template <int ENTRIES>
 struct Shared {
-    unsigned long long lists[LP_WARPS][ENTRIES ? ENTRIES * 32 : 1];   // each warp's, in order
-    unsigned long long floor;                          // an entry that the row's k-th best is known to be or to come before
+    unsigned long long lists[LP_WARPS][ENTRIES ? ENTRIES * 32 : 1];   // each warp's, in order, at the end
+    uint32_t reach[LP_WARPS];                          // each warp's ceil(top / 8)-th best key so far, 0: none yet
+};
+// Where the lanes of a warp leave a batch
+struct Stash {
+    uint4 bytes[32][4];
+    int first[32];                                     // the index of a lane's first value
 };
 
 // A warp's share of a row: batches `part`, part + parts, ...
 template <typename T, int ENTRIES, bool TEAM>
-__device__ __forceinline__ void lp_scan(const LogprobsParams& p, const T* row, int64_t label64, float& mine, int part, int parts, unsigned long long* queue,
+__device__ __forceinline__ void lp_scan(const LogprobsParams& p, const T* row, int64_t label64, float& mine, int part, int parts, Stash* stash,
                                         Shared<ENTRIES>* shared, Part& all, unsigned& before, Best<ENTRIES>& best) {
     constexpr int N = Vec<T>::N, VECS = 4, BATCH = 32 * VECS * N;
     const int lane = threadIdx.x & 31, n = p.classes;
@@ -260,9 +271,18 @@ __device__ __forceinline__ void lp_scan(const LogprobsParams& p, const T* row, i
     const int shift = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
     const int step = parts * BATCH;
     int first = part * BATCH - shift + lane * N;       // this lane's first element of the batch
-    Vec<T> v[VECS], ahead[VECS];
+    Vec<T> v[VECS];
+    auto load = [&](int b) {
+        if (b * BATCH >= shift && (b + 1) * BATCH - shift <= n) {   // (the same in all lanes)
+            const uint4* const at = reinterpret_cast<const uint4*>(row + first);
 #pragma unroll
-    for (int i = 0; i < VECS; i++) ahead[i].load(row, first + i * 32 * N, n);
+            for (int i = 0; i < VECS; i++) v[i].raw = __ldg(at + i * 32);
+        } else {
+#pragma unroll
+            for (int i = 0; i < VECS; i++) v[i].load(row, first + i * 32 * N, n);
+        }
+    };
+    load(part);
 
     const bool have = label64 >= 0 && label64 < n;
     const int label = have ? (int)label64 : -1;
@@ -270,6 +290,7 @@ __device__ __forceinline__ void lp_scan(const LogprobsParams& p, const T* row, i
     // classes before the label: those at least as large as it in front of it, those larger behind it
     const uint32_t mykey = order_key(mine);
     const float thr_front = pass_from(mykey), thr_behind = pass_above(mykey);
+    const auto many_front = Count<T>::threshold(thr_front), many_behind = Count<T>::threshold(thr_behind);
     const bool all_front = mine == -INFINITY, none_behind = mine != mine;   // (thresholds that would pass what is outside the row, or a NaN)
 
     all = Part{-INFINITY, 0.f, 0.f};
@@ -279,125 +300,112 @@ __device__ __forceinline__ void lp_scan(const LogprobsParams& p, const T* row, i
     for (int h = 0; h < ENTRIES; h++) best.e[h] = 0;
     float thr = __int_as_float(0x7fc00000);            // an alternative is what passes: not (v <= thr)
     bool fresh = true;                                 // the list has not been filled yet
-    const int batches = (int)(((long long)n + shift + BATCH - 1) / BATCH), rounds = (batches + parts - 1) / parts;
-    for (int round = 0, b = part; round < rounds; round++, b += parts) {
+    const int batches = (int)(((long long)n + shift + BATCH - 1) / BATCH);
+    for (int b = part; b < batches; b += parts) {
+        if (b != part) load(b);
+        const float half[2] = {vec_max(v[0], v[1]), vec_max(v[2], v[3])};
+        const float top = max_nan(half[0], half[1]);
+        const float to = fmaxf(all.m, top);        // (a NaN is passed over: it makes S one)
+        if (to > all.m) all.raise(to);
+        const float base = all.m == -INFINITY ? 0.f : all.m;
+        float2 s = make_float2(0.f, 0.f), w = s;
 #pragma unroll
-        for (int i = 0; i < VECS; i++) v[i] = ahead[i];
-        if (b + parts < batches)
+        for (int i = 0; i < VECS; i++)
 #pragma unroll
-            for (int i = 0; i < VECS; i++) ahead[i].load(row, first + step + i * 32 * N, n);
-        if (b < batches) {
-            const float half[2] = {vec_max(v[0], v[1]), vec_max(v[2], v[3])};
-            const float top = max_nan(half[0], half[1]);
-            const float to = fmaxf(all.m, top);        // (a NaN is passed over: it makes S one)
-            if (to > all.m) all.raise(to);
-            const float base = all.m == -INFINITY ? 0.f : all.m;
-            float2 s = make_float2(0.f, 0.f), w = s;
-#pragma unroll
-            for (int i = 0; i < VECS; i++)
-#pragma unroll
-                for (int e = 0; e < N; e += 2) {
-                    float2 t = two_mul(two_add(make_float2(v[i].value(e), v[i].value(e + 1)), make_float2(-base, -base)), make_float2(LP_LOG2E, LP_LOG2E));
-                    t = make_float2(max_nan(t.x, LP_FLOOR), max_nan(t.y, LP_FLOOR));
-                    const float2 x = make_float2(exp2_fast(t.x), exp2_fast(t.y));
-                    s = two_add(s, x);
-                    w = two_fma(t, x, w);
-                }
-            all.s += s.x + s.y;
-            all.w += w.x + w.y;
-
-            if (have) {
-#pragma unroll
-                for (int i = 0; i < VECS; i++) {
-                    const int at = first + i * 32 * N;
-                    const bool front = at + N <= label;
-                    unsigned c = vec_count(v[i], front ? thr_front : thr_behind);
-                    if (front ? all_front : none_behind) c = 0;
-                    if (at <= label && !front) {       // the label's own vector
-                        c = 0;
-#pragma unroll
-                        for (int e = 0; e < N; e++) {
-                            const bool inside = at + e >= 0 && at + e < n;
-                            if (inside && at + e < label && !all_front) c += !(v[i].value(e) <= thr_front);
-                            if (inside && at + e > label && !none_behind) c += !(v[i].value(e) <= thr_behind);
-                        }
-                    }
-                    before += c;
-                }
+            for (int e = 0; e < N; e += 2) {
+                float2 t = two_mul(two_add(make_float2(v[i].value(e), v[i].value(e + 1)), make_float2(-base, -base)), make_float2(LP_LOG2E, LP_LOG2E));
+                t = make_float2(max_nan(t.x, LP_FLOOR), max_nan(t.y, LP_FLOOR));
+                const float2 x = make_float2(exp2_fast(t.x), exp2_fast(t.y));
+                s = two_add(s, x);
+                w = two_fma(t, x, w);
             }
+        all.s += s.x + s.y;
+        all.w += w.x + w.y;
 
-            if (ENTRIES && __any_sync(0xffffffffu, !(top <= thr))) {
-                if (fresh || __popc(__ballot_sync(0xffffffffu, !(top <= thr))) > 8) {
-                    // the top-th largest of the 64 half-lane maxima: as many classes are that large
-                    uint32_t a = order_key(half[0]), c = order_key(half[1]), kth = 0;
-                    for (int k = 0; k < p.top; k++) {
-                        const uint32_t mx = max(a, c);
-                        kth = __reduce_max_sync(0xffffffffu, mx);
-                        const int who = __ffs(__ballot_sync(0xffffffffu, mx == kth)) - 1;
-                        if (lane == who) { if (a >= c) a = 0; else c = 0; }
-                    }
-                    if (kth > 0x007fffffu) {           // (-inf may stand for what is outside the row)
-                        const float t = pass_from(kth);
-                        if (!(t <= thr)) thr = t;
-                    }
-                }
-                unsigned long long last = best.at(p.top - 1);
-#pragma unroll 1
-                for (int i = 0; i < VECS; i++) {
-                    Vec<T> u = v[0];
+        if (have) {
+            Count<T> c;
 #pragma unroll
-                    for (int k = 1; k < VECS; k++)
-                        if (i == k) u = v[k];
-                    if (!__any_sync(0xffffffffu, !(vec_max(u, u) <= thr))) continue;
-                    int count = 0;
+            for (int i = 0; i < VECS; i++) c.add(v[i], first + i * 32 * N + N <= label ? many_front : many_behind);
+            int count = c.total();
+            // the label's own vector, and labels whose thresholds are of no use: one by one
+            if (all_front || none_behind || (unsigned)(label - first) < (unsigned)((VECS - 1) * 32 * N + N)) {
+                count = 0;
+#pragma unroll
+                for (int i = 0; i < VECS; i++)
 #pragma unroll
                     for (int e = 0; e < N; e++) {
                         const int at = first + i * 32 * N + e;
-                        const bool hit = !(u.value(e) <= thr) && at >= 0 && at < n;
-                        const uint32_t mask = __ballot_sync(0xffffffffu, hit);
-                        if (hit) queue[count + __popc(mask & ((1u << lane) - 1))] = (unsigned long long)order_key(u.value(e)) << 32 | (uint32_t)~at;
-                        count += __popc(mask);
+                        if (at >= 0 && at < n && (at < label ? !all_front && !(v[i].value(e) <= thr_front) : at > label && !none_behind && !(v[i].value(e) <= thr_behind))) count++;
                     }
-                    __syncwarp();
+            }
+            before += count;
+        }
+
+        if (ENTRIES) {
+            if (TEAM) {
+                const uint32_t key = __reduce_min_sync(0xffffffffu, lane < LP_WARPS ? *(volatile uint32_t*)&shared->reach[lane] : 0xffffffffu);
+                if (key > 0x007fffffu) {           // (what equals it may still come before it)
+                    const float t = pass_from(key);
+                    if (!(t <= thr)) thr = t;
+                }
+            }
+            uint32_t hot = __ballot_sync(0xffffffffu, !(top <= thr));
+            if (hot && (fresh || __popc(hot) > 8)) {
+                // the top-th largest of the 64 half-lane maxima: as many classes are that large
+                uint32_t a = order_key(half[0]), c = order_key(half[1]), kth = 0;
+                for (int k = 0; k < p.top; k++) {
+                    const uint32_t mx = max(a, c);
+                    kth = __reduce_max_sync(0xffffffffu, mx);
+                    const int who = __ffs(__ballot_sync(0xffffffffu, mx == kth)) - 1;
+                    if (lane == who) { if (a >= c) a = 0; else c = 0; }
+                }
+                if (kth > 0x007fffffu) {           // (-inf may stand for what is outside the row)
+                    const float t = pass_from(kth);
+                    if (!(t <= thr)) thr = t;
+                }
+                hot = __ballot_sync(0xffffffffu, !(top <= thr));
+            }
+            if (hot) {
+                if (hot >> lane & 1) {
+                    const int slot = __popc(hot & ((1u << lane) - 1));
+#pragma unroll
+                    for (int i = 0; i < VECS; i++) stash->bytes[slot][i] = v[i].raw;
+                    stash->first[slot] = first;
+                }
+                __syncwarp();
+                unsigned long long last = best.at(p.top - 1);
+                constexpr int AT_ONCE = 32 / (VECS * N);   // lanes' batches that a warp looks at together
+                const int nhot = __popc(hot), j = lane % (VECS * N);
 #pragma unroll 1
-                    for (int q = 0; q < count; q++) {
-                        const unsigned long long x = queue[q];
-                        if (x > last) {
-                            best.insert(x);
+                for (int q = 0; q < nhot; q += AT_ONCE) {
+                    const int slot = q + lane / (VECS * N);
+                    unsigned long long x = 0;
+                    if (slot < nhot) {
+                        const float u = to_f32(reinterpret_cast<const T*>(stash->bytes[slot])[j]);
+                        const int at = stash->first[slot] + j / N * 32 * N + j % N;
+                        if (!(u <= thr) && (unsigned)at < (unsigned)n) x = (unsigned long long)order_key(u) << 32 | (uint32_t)~at;
+                    }
+                    for (uint32_t mask = __ballot_sync(0xffffffffu, x > last); mask; mask &= mask - 1) {
+                        const unsigned long long y = __shfl_sync(0xffffffffu, x, __ffs(mask) - 1);
+                        if (y > last) {
+                            best.insert(y);
                             last = best.at(p.top - 1);
                         }
                     }
-                    __syncwarp();
-                    if (last) {                        // in a warp's own order what equals it comes after it
-                        fresh = false;
-                        const float t = pass_above((uint32_t)(last >> 32));
-                        if (!(t <= thr)) thr = t;
-                    }
+                }
+                __syncwarp();
+                if (last) {                        // in a warp's own order what equals it comes after it
+                    fresh = false;
+                    const float t = pass_above((uint32_t)(last >> 32));
+                    if (!(t <= thr)) thr = t;
+                }
+                if (TEAM) {
+                    const uint32_t key = (uint32_t)(best.at((p.top + LP_WARPS - 1) / LP_WARPS - 1) >> 32);
+                    if (lane == 0) *(volatile uint32_t*)&shared->reach[threadIdx.x >> 5] = key;
                 }
             }
         }
         first += step;
-        // the k-th best of all eight warps so far, after 1, 2, 4, ... rounds
-        if (TEAM && ENTRIES && round + 1 < rounds && (round & (round + 1)) == 0) {
-#pragma unroll
-            for (int h = 0; h < ENTRIES; h++) shared->lists[threadIdx.x >> 5][h * 32 + lane] = best.e[h];
-            __syncthreads();
-            for (int i = threadIdx.x; i < LP_WARPS * p.top; i += LP_WARPS * 32) {
-                const unsigned long long x = shared->lists[i / p.top][i % p.top];
-                int at = 0;
-                if (x)
-                    for (int k = 0; k < LP_WARPS; k++) at += entries_before(shared->lists[k], p.top, x);
-                if (x && at == p.top - 1) shared->floor = x;
-            }
-            __syncthreads();
-            const unsigned long long f = shared->floor;
-            const uint32_t key = (uint32_t)(f >> 32);
-            if (key > 0x007fffffu) {                   // its equals pass only while they may come before it
-                const bool later = (b + parts) * BATCH - shift > (int)~(uint32_t)f;
-                const float t = later ? pass_above(key) : pass_from(key);
-                if (!(t <= thr)) thr = t;
-            }
-        }
     }
     // the lanes' parts
 #pragma unroll
@@ -413,8 +421,8 @@ __device__ __forceinline__ void lp_scan(const LogprobsParams& p, const T* row, i
 
 // a warp per row
 template <typename T, int ENTRIES>
-__global__ void __launch_bounds__(LP_WARPS * 32, 3) logprobs_warp_kernel(const LogprobsParams p) {
-    __shared__ unsigned long long queue[ENTRIES ? LP_WARPS : 1][32 * Vec<T>::N];
+__global__ void __launch_bounds__(LP_WARPS * 32, 4) logprobs_warp_kernel(const LogprobsParams p) {
+    __shared__ Stash stash[ENTRIES ? LP_WARPS : 1];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const long long row = (long long)blockIdx.x * LP_WARPS + warp;
     grid_dependency_wait();
@@ -424,7 +432,7 @@ __global__ void __launch_bounds__(LP_WARPS * 32, 3) logprobs_warp_kernel(const L
     Part all;
     unsigned before;
     Best<ENTRIES> best;
-    lp_scan<T, ENTRIES, false>(p, static_cast<const T*>(p.logits) + row * p.ld, label, mine, 0, 1, queue[ENTRIES ? warp : 0], nullptr, all, before, best);
+    lp_scan<T, ENTRIES, false>(p, static_cast<const T*>(p.logits) + row * p.ld, label, mine, 0, 1, &stash[ENTRIES ? warp : 0], nullptr, all, before, best);
     if (lane == 0) lp_write(p, row, label, mine, all, before);
     if (ENTRIES)
 #pragma unroll
@@ -434,16 +442,16 @@ __global__ void __launch_bounds__(LP_WARPS * 32, 3) logprobs_warp_kernel(const L
 
 // a cluster of CTAs (one, where rows are many) per row
 template <typename T, int ENTRIES>
-__global__ void __launch_bounds__(LP_WARPS * 32, 3) logprobs_team_kernel(const LogprobsParams p, const int ctas) {
+__global__ void __launch_bounds__(LP_WARPS * 32, 4) logprobs_team_kernel(const LogprobsParams p, const int ctas) {
     constexpr int LIST = ENTRIES ? ENTRIES * 32 : 1;
-    __shared__ unsigned long long queue[ENTRIES ? LP_WARPS : 1][32 * Vec<T>::N];
+    __shared__ Stash stash[ENTRIES ? LP_WARPS : 1];
     __shared__ Shared<ENTRIES> shared;
     __shared__ unsigned long long merged[LIST], gathered[LP_MAX_CLUSTER * LIST];
     __shared__ Part parts[LP_WARPS], part_s;
     __shared__ unsigned before_s[LP_WARPS], before_cta;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = blockIdx.x % ctas;
     const long long row = blockIdx.x / ctas;
-    if (threadIdx.x == 0) shared.floor = 0;
+    if (threadIdx.x < LP_WARPS) shared.reach[threadIdx.x] = 0;
     __syncthreads();
     grid_dependency_wait();
     const int64_t label = p.labels ? p.labels[row] : -1;
@@ -451,24 +459,36 @@ __global__ void __launch_bounds__(LP_WARPS * 32, 3) logprobs_team_kernel(const L
     Part all;
     unsigned before;
     Best<ENTRIES> best;
-    lp_scan<T, ENTRIES, true>(p, static_cast<const T*>(p.logits) + row * p.ld, label, mine, warp * ctas + rank, LP_WARPS * ctas, queue[ENTRIES ? warp : 0], &shared, all,
+    lp_scan<T, ENTRIES, true>(p, static_cast<const T*>(p.logits) + row * p.ld, label, mine, warp * ctas + rank, LP_WARPS * ctas, &stash[ENTRIES ? warp : 0], &shared, all,
                               before, best);
     if (lane == 0) { parts[warp] = all; before_s[warp] = before; }
     if (ENTRIES)
 #pragma unroll
         for (int h = 0; h < ENTRIES; h++) shared.lists[warp][h * 32 + lane] = best.e[h];
     __syncthreads();
-    all = parts[0];
-    before = before_s[0];
-#pragma unroll
-    for (int i = 1; i < LP_WARPS; i++) { all.join(parts[i]); before += before_s[i]; }
     // an entry's place: how many of the others come before it (no two are alike; 0 stands for none)
     auto place = [&](const unsigned long long* entries, int count, unsigned long long x) {
         int better = 0;
         for (int i = 0; i < count; i++) better += entries_before(entries + i * LIST, p.top, x);
         return better;
     };
+    if (warp == 0) {
+        all = parts[lane % LP_WARPS];
+        before = before_s[lane % LP_WARPS];
+#pragma unroll
+        for (int d = LP_WARPS / 2; d; d >>= 1) {
+            Part o;
+            o.m = __shfl_xor_sync(0xffffffffu, all.m, d);
+            o.s = __shfl_xor_sync(0xffffffffu, all.s, d);
+            o.w = __shfl_xor_sync(0xffffffffu, all.w, d);
+            all.join(o);
+            before += __shfl_xor_sync(0xffffffffu, before, d);
+        }
+        if (lane == 0) { part_s = all; before_cta = before; }
+        if (lane == 0 && ctas == 1) lp_write(p, row, label, mine, all, before);
+    }
     if (ENTRIES) {
+        // (at least `top` entries of a row's only CTA; of a cluster's CTAs perhaps fewer)
         if (ctas > 1) {
             for (int i = threadIdx.x; i < LIST; i += LP_WARPS * 32) merged[i] = 0;
             __syncthreads();
@@ -476,17 +496,15 @@ __global__ void __launch_bounds__(LP_WARPS * 32, 3) logprobs_team_kernel(const L
         for (int i = threadIdx.x; i < LP_WARPS * p.top; i += LP_WARPS * 32) {
             const unsigned long long x = shared.lists[i / p.top][i % p.top];
             const int at = x ? place(&shared.lists[0][0], LP_WARPS, x) : p.top;
-            if (at < p.top) {
-                if (ctas > 1) merged[at] = x;
-                else lp_write_top(p, row, at, x, all);
-            }
+            if (at < p.top) merged[at] = x;
         }
     }
     if (ctas == 1) {
-        if (threadIdx.x == 0) lp_write(p, row, label, mine, all, before);
+        if (!ENTRIES) return;
+        __syncthreads();
+        if ((int)threadIdx.x < p.top) lp_write_top(p, row, threadIdx.x, merged[threadIdx.x], part_s);
         return;
     }
-    if (threadIdx.x == 0) { part_s = all; before_cta = before; }
     auto cluster_sync = [] { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); };
     __syncwarp();
     cluster_sync();
@@ -507,6 +525,8 @@ __global__ void __launch_bounds__(LP_WARPS * 32, 3) logprobs_team_kernel(const L
                 asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(x) : "r"(there(&merged[i % p.top], i / p.top)) : "memory");
                 gathered[i / p.top * LIST + i % p.top] = x;
             }
+        all = part_s;
+        before = before_cta;
         Part o[LP_MAX_CLUSTER];
         unsigned c[LP_MAX_CLUSTER];
 #pragma unroll
