@@ -314,7 +314,7 @@ def _here(*tensors):
     """The kernels run on the current device, on its current stream."""
     device = torch._C._cuda_getDevice()
     for t in tensors:
-        if t is not None and not (isinstance(t, torch.Tensor) and t.is_cuda and t.device.index == device):
+        if t is not None and t.get_device() != device:
             raise TypeError("expected CUDA tensors on the current device")
 
 
@@ -339,12 +339,12 @@ def _fp8_quantize(x, block_rows):
     pitch, blocks = (k + 15) // 16 * 16, (k + FP8_BLOCK - 1) // FP8_BLOCK
     q = torch.empty((rows, pitch), dtype=torch.float8_e4m3fn, device=x.device)
     if block_rows == 1:   # block by block: the order in which the product reads them
-        scales = torch.empty((blocks, rows), dtype=torch.float32, device=x.device).t()
-        steps = (1, rows)
+        scales = torch.empty_strided((rows, blocks), (1, rows), dtype=torch.float32, device=x.device)
+        step, block_step = 1, rows
     else:
         scales = torch.empty(((rows + block_rows - 1) // block_rows, blocks), dtype=torch.float32, device=x.device)
-        steps = (blocks, 1)
-    check(capi.load().dabnn_fp8_quantize(_ptr(x), kind, ld, _ptr(q), pitch, _ptr(scales), *steps, rows, k, block_rows, _stream()))
+        step, block_step = blocks, 1
+    check(capi.load().dabnn_fp8_quantize(x.data_ptr(), kind, ld, q.data_ptr(), pitch, scales.data_ptr(), step, block_step, rows, k, block_rows, _stream()))
     return (q if pitch == k else q[:, :k]), scales
 
 
@@ -372,8 +372,9 @@ def fp8_gemm(a, a_scales, b, b_scales, bias=None, out_dtype=torch.float32):
         raise TypeError("fp8_gemm: the result is fp32, fp16 or bf16")
     if a.dtype != torch.float8_e4m3fn or b.dtype != torch.float8_e4m3fn or a_scales.dtype != torch.float32 or b_scales.dtype != torch.float32:
         raise TypeError("fp8_gemm: expected float8_e4m3fn operands and fp32 scales")
-    lead = a.shape[:-1]
+    lead = None
     if a.dim() != 2:
+        lead = a.shape[:-1]
         a = a.unsqueeze(0) if a.dim() == 1 else a.flatten(0, -2)
         a_scales = a_scales.unsqueeze(0) if a_scales.dim() == 1 else a_scales.flatten(0, -2)
     if b.dim() != 2:
@@ -386,9 +387,9 @@ def fp8_gemm(a, a_scales, b, b_scales, bias=None, out_dtype=torch.float32):
     if bias is not None and (bias.dtype != torch.float32 or bias.shape != (n,) or not bias.is_contiguous()):
         raise TypeError("fp8_gemm: expected a contiguous fp32 bias of N values")
     c = torch.empty((m, n), dtype=out_dtype, device=a.device)
-    check(capi.load().dabnn_fp8_gemm(_ptr(a), lda, _ptr(a_scales), *a_scales.stride(), _ptr(b), ldb, _ptr(b_scales), *b_scales.stride(), _ptr(bias),
-                                     _ptr(c), kind, n, m, n, k, _stream()))
-    return c if len(lead) == 1 else c.unflatten(0, lead) if lead else c[0]
+    check(capi.load().dabnn_fp8_gemm(a.data_ptr(), lda, a_scales.data_ptr(), *a_scales.stride(), b.data_ptr(), ldb, b_scales.data_ptr(), *b_scales.stride(),
+                                     _ptr(bias), c.data_ptr(), kind, n, m, n, k, _stream()))
+    return c if lead is None else c.unflatten(0, lead) if lead else c[0]
 
 
 def logprobs(logits, labels=None, top=0):
@@ -401,16 +402,18 @@ def logprobs(logits, labels=None, top=0):
     if kind is None:
         raise TypeError("logprobs: expected fp32, fp16 or bf16")
     rows, classes, ld = _rows(logits, "logprobs")
-    lead, device = logits.shape[:-1], logits.device
+    lead = logits.shape[:-1]
     lp = rank = tlp = ti = None
     if labels is not None:
         if labels.dtype != torch.int64 or labels.shape != lead or not labels.is_contiguous():
             raise TypeError("logprobs: expected contiguous int64 labels, one for each row")
-        lp, rank = torch.empty(lead, dtype=torch.float32, device=device), torch.empty(lead, dtype=torch.int64, device=device)
-    entropy = torch.empty(lead, dtype=torch.float32, device=device)
+        rank, lp = torch.empty_like(labels), torch.empty_like(labels, dtype=torch.float32)
+        entropy = torch.empty_like(lp)
+    else:
+        entropy = logits.new_empty(lead, dtype=torch.float32)
     if top:
-        tlp, ti = (torch.empty((*lead, max(top, 0)), dtype=t, device=device) for t in (torch.float32, torch.int64))
-    check(capi.load().dabnn_logprobs(_ptr(logits), kind, ld, _ptr(labels), rows, classes, _ptr(lp), _ptr(rank), _ptr(entropy), _ptr(tlp),
+        tlp, ti = entropy.new_empty((*lead, max(top, 0))), logits.new_empty((*lead, max(top, 0)), dtype=torch.int64)
+    check(capi.load().dabnn_logprobs(logits.data_ptr(), kind, ld, _ptr(labels), rows, classes, _ptr(lp), _ptr(rank), entropy.data_ptr(), _ptr(tlp),
                                      _ptr(ti), top, _stream()))
     return lp, rank, entropy, tlp, ti
 

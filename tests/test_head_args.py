@@ -95,6 +95,9 @@ class _Cuda(torch.Tensor):
     def device(self):
         return torch.device("cuda", self.at)
 
+    def get_device(self):
+        return self.at
+
 
 @pytest.fixture
 def pretend(monkeypatch):
