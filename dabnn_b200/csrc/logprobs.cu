@@ -5,13 +5,13 @@
 //
 // Classes are ordered by value, larger first, equal ones (the two zeros are) by index, a NaN before everything.
 //
-// One pass over a row, no warp waiting for another: a lane keeps its own m, S, W (rescaled when its m grows) and its own count
-// of classes before the label; a warp keeps its best classes in order, one to a lane.  A batch of a warp - 64 bytes of each
-// lane - is looked at for alternatives only if some lane's maximum passes a threshold: the warp's k-th best, or the least of
-// the eight warps' ceil(k / 8)-th bests (k classes of the row reach that).  The lanes that pass leave their 64 bytes in shared
-// memory, where the warp looks at the values of one lane (two of fp32) at a time, inserting what belongs among the best.  The
-// first batch has no threshold yet: the k-th largest of the 64 half-lane maxima is one, since there are then at least k classes
-// that reach it.
+// One pass over a row: a lane keeps its own m, S, W (rescaled when its m grows) and its own count of classes before the label;
+// a warp keeps its best classes in order, one to a lane.  A batch of a warp - 64 bytes of each lane - is looked at for
+// alternatives only if some lane's maximum passes a threshold.  With r = ceil(k / 4), the fourth largest of the eight warps'
+// r-th best classes is one (4 r >= k classes reach it), and so is the warp's own k-th best.  A row's first batches have no best
+// classes yet: there the r-th largest of a warp's 64 half-lane maxima stands for its r-th best, and the warps meet once to
+// compare them.  The lanes that pass leave their 64 bytes in shared memory, where the warp looks at the values of one lane (two
+// of fp32) at a time, inserting what belongs among the best.
 //
 // A row is scored by one warp, or by a CTA of eight, or by a cluster of such CTAs where rows are few: the warps take the row's
 // batches in turn and their parts are joined at the end, lists of best classes by counting, for each entry, the better ones.
@@ -25,7 +25,8 @@
 
 namespace dabnn {
 
-constexpr int LP_WARPS = 8, LP_MAX_CLUSTER = 8;
+constexpr int LP_WARPS = 8, LP_MAX_CLUSTER = 8;        // warps of a CTA that share a row, CTAs of a cluster
+constexpr int LP_ROWS = 4;                             // warps of a CTA that have a row each
 constexpr float LP_LOG2E = 1.4426950408889634f, LP_LN2 = 0.6931471805599453f;
 constexpr float LP_FLOOR = -1e30f;                     // a difference below it has e^d = 0; keeps d e^d a number
 
@@ -253,8 +254,22 @@ __device__ __forceinline__ int entries_before(const unsigned long long* list, in
 template <int ENTRIES>
 struct Shared {
     unsigned long long lists[LP_WARPS][ENTRIES ? ENTRIES * 32 : 1];   // each warp's, in order, at the end
-    uint32_t reach[LP_WARPS];                          // each warp's ceil(top / 8)-th best key so far, 0: none yet
+    uint32_t reach[LP_WARPS];                          // a key that ceil(top / 4) classes of a warp reach, 0: none yet
 };
+// the fourth largest of the eight
+__device__ __forceinline__ uint32_t fourth_of(const uint32_t* reach) {
+    const volatile uint32_t* const r = reach;
+    const int lane = threadIdx.x & 31;
+    const uint32_t mine = lane < LP_WARPS ? r[lane] : 0;
+    int larger = 0;
+#pragma unroll
+    for (int i = 0; i < LP_WARPS; i++) {
+        const uint32_t o = __shfl_sync(0xffffffffu, mine, i);
+        larger += o > mine || (o == mine && i < lane);
+    }
+    return __shfl_sync(0xffffffffu, mine, __ffs(__ballot_sync(0xffffffffu, larger == 3 && lane < LP_WARPS)) - 1);
+}
+__device__ __forceinline__ void team_sync() { asm volatile("bar.sync 1, %0;" ::"n"(LP_WARPS * 32) : "memory"); }
 // Where the lanes of a warp leave a batch
 struct Stash {
     uint4 bytes[32][4];
@@ -266,7 +281,7 @@ template <typename T, int ENTRIES, bool TEAM>
 __device__ __forceinline__ void lp_scan(const LogprobsParams& p, const T* row, int64_t label64, float& mine, int part, int parts, Stash* stash,
                                         Shared<ENTRIES>* shared, Part& all, unsigned& before, Best<ENTRIES>& best) {
     constexpr int N = Vec<T>::N, VECS = 4, BATCH = 32 * VECS * N;
-    const int lane = threadIdx.x & 31, n = p.classes;
+    const int warp = uniform_warp(), lane = threadIdx.x & 31, n = p.classes;
     // vectors are counted from the 16-byte boundary at or below the row's first element, which is element `shift` there
     const int shift = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
     const int step = parts * BATCH;
@@ -284,13 +299,12 @@ __device__ __forceinline__ void lp_scan(const LogprobsParams& p, const T* row, i
     };
     load(part);
 
-    const bool have = label64 >= 0 && label64 < n;
-    const int label = have ? (int)label64 : -1;
+    const bool have = __shfl_sync(0xffffffffu, label64 >= 0 && label64 < n, 0);
+    const int label = __shfl_sync(0xffffffffu, have ? (int)label64 : -1, 0);   // (known to be the same in all lanes)
     mine = have ? to_f32(row[label]) : 0.f;
     // classes before the label: those at least as large as it in front of it, those larger behind it
     const uint32_t mykey = order_key(mine);
-    const float thr_front = pass_from(mykey), thr_behind = pass_above(mykey);
-    const auto many_front = Count<T>::threshold(thr_front), many_behind = Count<T>::threshold(thr_behind);
+    const auto many_front = Count<T>::threshold(pass_from(mykey)), many_behind = Count<T>::threshold(pass_above(mykey));
     const bool all_front = mine == -INFINITY, none_behind = mine != mine;   // (thresholds that would pass what is outside the row, or a NaN)
 
     all = Part{-INFINITY, 0.f, 0.f};
@@ -299,8 +313,9 @@ __device__ __forceinline__ void lp_scan(const LogprobsParams& p, const T* row, i
 #pragma unroll
     for (int h = 0; h < ENTRIES; h++) best.e[h] = 0;
     float thr = __int_as_float(0x7fc00000);            // an alternative is what passes: not (v <= thr)
-    bool fresh = true;                                 // the list has not been filled yet
+    const int reach_at = (p.top + 3) / 4 - 1;
     const int batches = (int)(((long long)n + shift + BATCH - 1) / BATCH);
+    if (TEAM && ENTRIES && part >= batches) team_sync();   // nothing to do but to let the others pass
     for (int b = part; b < batches; b += parts) {
         if (b != part) load(b);
         const float half[2] = {vec_max(v[0], v[1]), vec_max(v[2], v[3])};
@@ -329,6 +344,7 @@ __device__ __forceinline__ void lp_scan(const LogprobsParams& p, const T* row, i
             int count = c.total();
             // the label's own vector, and labels whose thresholds are of no use: one by one
             if (all_front || none_behind || (unsigned)(label - first) < (unsigned)((VECS - 1) * 32 * N + N)) {
+                const float thr_front = pass_from(order_key(mine)), thr_behind = pass_above(order_key(mine));
                 count = 0;
 #pragma unroll
                 for (int i = 0; i < VECS; i++)
@@ -342,27 +358,35 @@ __device__ __forceinline__ void lp_scan(const LogprobsParams& p, const T* row, i
         }
 
         if (ENTRIES) {
-            if (TEAM) {
-                const uint32_t key = __reduce_min_sync(0xffffffffu, lane < LP_WARPS ? *(volatile uint32_t*)&shared->reach[lane] : 0xffffffffu);
-                if (key > 0x007fffffu) {           // (what equals it may still come before it)
-                    const float t = pass_from(key);
-                    if (!(t <= thr)) thr = t;
-                }
-            }
-            uint32_t hot = __ballot_sync(0xffffffffu, !(top <= thr));
-            if (hot && (fresh || __popc(hot) > 8)) {
-                // the top-th largest of the 64 half-lane maxima: as many classes are that large
-                uint32_t a = order_key(half[0]), c = order_key(half[1]), kth = 0;
-                for (int k = 0; k < p.top; k++) {
+            // the nth largest of the 64 half-lane maxima: as many classes are that large
+            auto nth_maximum = [&](int nth) {
+                uint32_t a = order_key(half[0]), c = order_key(half[1]), key = 0;
+                for (int k = 0; k < nth; k++) {
                     const uint32_t mx = max(a, c);
-                    kth = __reduce_max_sync(0xffffffffu, mx);
-                    const int who = __ffs(__ballot_sync(0xffffffffu, mx == kth)) - 1;
+                    key = __reduce_max_sync(0xffffffffu, mx);
+                    const int who = __ffs(__ballot_sync(0xffffffffu, mx == key)) - 1;
                     if (lane == who) { if (a >= c) a = 0; else c = 0; }
                 }
-                if (kth > 0x007fffffu) {           // (-inf may stand for what is outside the row)
-                    const float t = pass_from(kth);
+                return key;
+            };
+            auto raise_to = [&](uint32_t key) {        // (-inf may stand for what is outside the row)
+                if (key > 0x007fffffu) {
+                    const float t = pass_from(key);    // what equals it may still come before it
                     if (!(t <= thr)) thr = t;
                 }
+            };
+            if (TEAM && b == part) {
+                const uint32_t key = nth_maximum(reach_at + 1);
+                if (lane == 0) shared->reach[warp] = key;
+                team_sync();
+            }
+            uint32_t hot = __ballot_sync(0xffffffffu, !(top <= thr));
+            if (TEAM && hot) {
+                raise_to(fourth_of(shared->reach));
+                hot = __ballot_sync(0xffffffffu, !(top <= thr));
+            }
+            if (__popc(hot) > 8) {
+                raise_to(nth_maximum(p.top));
                 hot = __ballot_sync(0xffffffffu, !(top <= thr));
             }
             if (hot) {
@@ -395,13 +419,13 @@ __device__ __forceinline__ void lp_scan(const LogprobsParams& p, const T* row, i
                 }
                 __syncwarp();
                 if (last) {                        // in a warp's own order what equals it comes after it
-                    fresh = false;
                     const float t = pass_above((uint32_t)(last >> 32));
                     if (!(t <= thr)) thr = t;
                 }
                 if (TEAM) {
-                    const uint32_t key = (uint32_t)(best.at((p.top + LP_WARPS - 1) / LP_WARPS - 1) >> 32);
-                    if (lane == 0) *(volatile uint32_t*)&shared->reach[threadIdx.x >> 5] = key;
+                    const uint32_t key = (uint32_t)(best.at(reach_at) >> 32);
+                    volatile uint32_t* const mine_s = &shared->reach[warp];
+                    if (lane == 0 && key > *mine_s) *mine_s = key;
                 }
             }
         }
@@ -421,10 +445,10 @@ __device__ __forceinline__ void lp_scan(const LogprobsParams& p, const T* row, i
 
 // a warp per row
 template <typename T, int ENTRIES>
-__global__ void __launch_bounds__(LP_WARPS * 32, 4) logprobs_warp_kernel(const LogprobsParams p) {
-    __shared__ Stash stash[ENTRIES ? LP_WARPS : 1];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const long long row = (long long)blockIdx.x * LP_WARPS + warp;
+__global__ void __launch_bounds__(LP_ROWS * 32, 7) logprobs_warp_kernel(const LogprobsParams p) {
+    __shared__ Stash stash[ENTRIES ? LP_ROWS : 1];
+    const int warp = uniform_warp(), lane = threadIdx.x & 31;
+    const long long row = (long long)blockIdx.x * LP_ROWS + warp;
     grid_dependency_wait();
     if (row >= p.rows) return;
     const int64_t label = p.labels ? p.labels[row] : -1;
@@ -449,7 +473,7 @@ __global__ void __launch_bounds__(LP_WARPS * 32, 4) logprobs_team_kernel(const L
     __shared__ unsigned long long merged[LIST], gathered[LP_MAX_CLUSTER * LIST];
     __shared__ Part parts[LP_WARPS], part_s;
     __shared__ unsigned before_s[LP_WARPS], before_cta;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = blockIdx.x % ctas;
+    const int warp = uniform_warp(), lane = threadIdx.x & 31, rank = blockIdx.x % ctas;
     const long long row = blockIdx.x / ctas;
     if (threadIdx.x < LP_WARPS) shared.reach[threadIdx.x] = 0;
     __syncthreads();
@@ -552,12 +576,13 @@ __global__ void __launch_bounds__(LP_WARPS * 32, 4) logprobs_team_kernel(const L
     cluster_sync();                                    // no CTA leaves while its part is being read
 }
 
-// Rows of one batch have a warp each, and so do those of up to 4096 classes where there are rows for every scheduler; others a
-// CTA, or as many CTAs (up to 8) as keep the SMs busy and find a batch for each of their warps.
+// Rows of one batch have a warp each; so do those of up to 4096 classes where every scheduler finds a row, and all where there
+// are 24 rows for an SM (4096 rows of 65536 bf16, top 8: 137 us with a warp each, 195 with a CTA; 1024 rows: 53 with a CTA).
+// Others a CTA, or as many CTAs (up to 8) as keep the SMs busy and find a batch for each of their warps.
 template <typename T, int ENTRIES>
 static int lp_launch(const LogprobsParams& p, cudaStream_t stream) {
-    if (p.classes <= 128 * Vec<T>::N || (p.classes <= 4096 && p.rows >= 4 * sm_count())) {
-        DABNN_CUDA_OK(launch_overlapped(logprobs_warp_kernel<T, ENTRIES>, dim3((unsigned)(((long long)p.rows + LP_WARPS - 1) / LP_WARPS)), dim3(LP_WARPS * 32), 0, stream, p));
+    if (p.classes <= 128 * Vec<T>::N || (p.classes <= 4096 && p.rows >= 4 * sm_count()) || p.rows >= 24 * sm_count()) {
+        DABNN_CUDA_OK(launch_overlapped(logprobs_warp_kernel<T, ENTRIES>, dim3((unsigned)(((long long)p.rows + LP_ROWS - 1) / LP_ROWS)), dim3(LP_ROWS * 32), 0, stream, p));
         return DABNN_OK;
     }
     int ctas = 1;
