@@ -198,7 +198,8 @@ static int f8_splits(long long ntiles, int nkb) {
 }
 
 template <int NT, bool SPLIT, typename T>
-static int f8_launch(const Fp8Params& p, int splits, const CUtensorMap& lane_map, const CUtensorMap& col_map, cudaStream_t stream) {
+static int f8_launch(const Fp8Params& p, int splits, const CUtensorMap& lane_map, const CUtensorMap& col_map, const CUtensorMap& out_map,
+                     cudaStream_t stream) {
     using Cfg = Fp8Cfg<NT>;
     auto kern = fp8_gemm_kernel<NT, SPLIT, T>;
     static thread_local int ready_device = -1, resident = 0;   // teams that run at once
@@ -235,7 +236,7 @@ static int f8_launch(const Fp8Params& p, int splits, const CUtensorMap& lane_map
         attr[n++].val.programmaticStreamSerializationAllowed = 1;
     }
     cfg.numAttrs = n;
-    DABNN_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, p, splits, lane_map, col_map));
+    DABNN_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, p, splits, lane_map, col_map, out_map));
     return DABNN_OK;
 }
 
@@ -247,7 +248,6 @@ static int f8_gemm(Fp8Params p, const uint8_t* a, long long lda, const uint8_t* 
     DABNN_REQUIRE(ntiles < (1ll << 30), DABNN_ERR_SHAPE, "fp8_gemm: too many outputs");
     p.ntiles = (int)ntiles;
     p.nkb = (k + F8_BLOCK - 1) / F8_BLOCK;
-    p.vec = aligned_to(p.c, 32) && (p.M == 1 || p.ldc * sizeof(T) % 32 == 0);
     CUtensorMap w_map{}, x_map{};
     if (k > 0) {   // a single row's pitch is of no account, but the descriptor wants one
         const unsigned long long whole = ((unsigned long long)k + 15) / 16 * 16;
@@ -257,13 +257,20 @@ static int f8_gemm(Fp8Params p, const uint8_t* a, long long lda, const uint8_t* 
         DABNN_REQUIRE(make_u8_tensor_map(&w_map, b, 2, wdims, wpitch, wbox) && make_u8_tensor_map(&x_map, a, 2, xdims, xpitch, xbox), DABNN_ERR_CUDA,
                       "fp8_gemm: cannot make a tensor map (no CUDA device, or a pitch beyond 2^40)");
     }
+    CUtensorMap out_map{};
+    p.tma_out = 0;
+    if (nt > 64 && aligned_to(p.c, 16) && p.ldc * sizeof(T) % 16 == 0 && (unsigned long long)p.ldc * sizeof(T) < (1ull << 40) && p.N * sizeof(T) < INT_MAX) {
+        const unsigned long long dims[2] = {p.N * sizeof(T), (unsigned long long)p.M}, pitch[1] = {p.ldc * sizeof(T)};
+        const unsigned box[2] = {128, 32};
+        p.tma_out = make_u8_tensor_map(&out_map, static_cast<const unsigned char*>(p.c), 2, dims, pitch, box);
+    }
     const int splits = nt <= 64 ? f8_splits(ntiles, p.nkb) : 1;
     switch (nt) {
-        case 16: return splits > 1 ? f8_launch<16, true, T>(p, splits, w_map, x_map, stream) : f8_launch<16, false, T>(p, 1, w_map, x_map, stream);
-        case 32: return splits > 1 ? f8_launch<32, true, T>(p, splits, w_map, x_map, stream) : f8_launch<32, false, T>(p, 1, w_map, x_map, stream);
-        case 64: return splits > 1 ? f8_launch<64, true, T>(p, splits, w_map, x_map, stream) : f8_launch<64, false, T>(p, 1, w_map, x_map, stream);
-        case 128: return f8_launch<128, false, T>(p, 1, x_map, w_map, stream);
-        default: return f8_launch<256, false, T>(p, 1, x_map, w_map, stream);
+        case 16: return splits > 1 ? f8_launch<16, true, T>(p, splits, w_map, x_map, out_map, stream) : f8_launch<16, false, T>(p, 1, w_map, x_map, out_map, stream);
+        case 32: return splits > 1 ? f8_launch<32, true, T>(p, splits, w_map, x_map, out_map, stream) : f8_launch<32, false, T>(p, 1, w_map, x_map, out_map, stream);
+        case 64: return splits > 1 ? f8_launch<64, true, T>(p, splits, w_map, x_map, out_map, stream) : f8_launch<64, false, T>(p, 1, w_map, x_map, out_map, stream);
+        case 128: return f8_launch<128, false, T>(p, 1, x_map, w_map, out_map, stream);
+        default: return f8_launch<256, false, T>(p, 1, x_map, w_map, out_map, stream);
     }
 }
 

@@ -27,6 +27,7 @@ namespace dabnn {
 constexpr int F8_BLOCK = 128;
 constexpr int F8_L_BYTES = 128 * F8_BLOCK;            // the lane operand of a stage
 constexpr int F8_MAX_SPLIT = 8;
+constexpr int F8_OUT_BYTES = 32 * 128;                // where a warp leaves 32 rows of 128 bytes of the result for a tensor store
 constexpr int F8_GROUPS = 2, F8_GROUP = 4;            // the ring of factors: groups of blocks, fetched and handed over together
 
 __device__ int g_fp8_status;   // 0 = ok; 51 - 55 as above
@@ -37,7 +38,7 @@ struct Fp8Params {
     void* c;
     int M, N, nkb;                                     // activation rows, weight rows, blocks of K
     int tiles_n, ntiles;                               // tiles along the weight rows; all tiles
-    int vec;                                           // rows of c begin on 32-byte boundaries
+    int tma_out;                                       // rows of c begin on 16-byte boundaries: tensor stores
 };
 
 template <int NT>
@@ -49,9 +50,10 @@ struct Fp8Cfg {                                        // NT: columns of a tile
     static constexpr int FACTORS = NT;      // of a block: one per column / per lane and 128 columns
     static constexpr int COL_ROWS = PAIR ? NT / 2 : NT;  // rows of the column operand that a CTA loads
     static constexpr int STAGE_BYTES = F8_L_BYTES + COL_ROWS * F8_BLOCK;
-    static constexpr int STAGES = NT <= 32 ? 5 : NT == 64 ? 4 : 6;
+    static constexpr int STAGES = NT <= 32 ? 5 : NT == 64 ? 4 : NT == 128 ? 5 : 4;
+    static constexpr int OUT_BYTES = FEW ? 0 : EPI_WARPS * F8_OUT_BYTES;
     static constexpr int CTAS_PER_SM = FEW ? 2 : 1;
-    static constexpr int SMEM = 1024 + STAGES * STAGE_BYTES;
+    static constexpr int SMEM = 1024 + STAGES * STAGE_BYTES + OUT_BYTES;
 };
 
 // A bounded wait of a whole warp
@@ -130,13 +132,13 @@ __device__ __forceinline__ void f8_cluster_sync() {
 // SPLIT: the CTAs of a cluster share one tile (the grid then has one cluster per tile); otherwise a CTA walks the tiles
 template <int NT, bool SPLIT, typename T>
 __global__ void __launch_bounds__(Fp8Cfg<NT>::THREADS, Fp8Cfg<NT>::CTAS_PER_SM)
-    fp8_gemm_kernel(const Fp8Params p, const int splits, const __grid_constant__ CUtensorMap lane_map, const __grid_constant__ CUtensorMap col_map) {
+    fp8_gemm_kernel(const Fp8Params p, const int splits, const __grid_constant__ CUtensorMap lane_map, const __grid_constant__ CUtensorMap col_map,
+                    const __grid_constant__ CUtensorMap out_map) {
     using Cfg = Fp8Cfg<NT>;
     extern __shared__ unsigned char smem_dyn[];
     __shared__ __align__(8) uint64_t bar_full[Cfg::STAGES], bar_empty[Cfg::STAGES], bar_acc_full[2], bar_acc_empty[2];
     __shared__ __align__(8) uint64_t bar_factor_full[F8_GROUPS], bar_factor_empty[F8_GROUPS];
     __shared__ __align__(16) float factors[F8_GROUPS][F8_GROUP][Cfg::FACTORS];
-    __shared__ __align__(32) float scratch[Cfg::FEW ? 1 : Cfg::EPI_WARPS][32 * 8];   // to turn 32 rows of 32 bytes over, for rows of c off a boundary
     __shared__ uint32_t tmem_base_s;
     __shared__ int s_abort;
 
@@ -366,50 +368,67 @@ __global__ void __launch_bounds__(Fp8Cfg<NT>::THREADS, Fp8Cfg<NT>::CTAS_PER_SM)
                     }
                 }
             } else {
-                // a thread has neighbouring outputs of its row: 32 bytes at a time
-                constexpr int W = 32 / (int)sizeof(T);
-                const int m = m0 + lane;
-                T* const out = static_cast<T*>(p.c) + m * p.ldc + n0;
-                if (p.bias) {                          // through shared memory: a warp's columns are the same in all its lanes
-                    const uint32_t mine = smem_u32(scratch[ew]);
+                // A thread has neighbouring outputs of its row: 128 bytes of each of the warp's rows go to shared memory in the
+                // swizzled layout of a tensor store, which writes whole lines while the warp goes on (stores from registers, 32
+                // bytes of 32 rows each, held the next tile up for 5000 cycles: 8192 x 8192 x 4096 in 243 us).
+                const uint32_t out = stage0 + Cfg::STAGES * Cfg::STAGE_BYTES + ew * F8_OUT_BYTES;
+                auto stored = [] {                     // the last store has read its bytes
+                    asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
                     __syncwarp();
+                };
+                stored();
+                if (p.bias) {                          // through shared memory: a warp's columns are the same in all its lanes
 #pragma unroll
-                    for (int e = 0; e < Cfg::COLS; e += 32) scratch[ew][e + lane] = __ldg(p.bias + min(n0 + e + lane, p.N - 1));
+                    for (int e = 0; e < Cfg::COLS; e += 32)
+                        asm volatile("st.shared.f32 [%0], %1;" ::"r"(out + (e + lane) * 4), "f"(__ldg(p.bias + min(n0 + e + lane, p.N - 1))) : "memory");
                     __syncwarp();
 #pragma unroll
                     for (int e = 0; e < Cfg::COLS; e += 4) {
-                        const float4 b = lds128f(mine + e * 4);
+                        const float4 b = lds128f(out + e * 4);
                         sum[e / 2].x += b.x; sum[e / 2].y += b.y; sum[e / 2 + 1].x += b.z; sum[e / 2 + 1].y += b.w;
                     }
+                    __syncwarp();
                 }
+                constexpr int W = 128 / (int)sizeof(T);
 #pragma unroll
                 for (int h = 0; h < Cfg::COLS; h += W) {
-                    const int left = p.N - n0 - h;     // the same in all lanes
-                    if (left <= 0) break;
-                    alignas(32) T o[W];
+                    if (h) stored();
 #pragma unroll
-                    for (int e = 0; e < W; e++) o[e] = from_f32<T>(sum_of(h + e));
-                    const uint4 *lo = reinterpret_cast<const uint4*>(o), *hi = lo + 1;
-                    if (p.vec && left >= W) {
-                        if (m < p.M)
-                            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out + h), "r"(lo->x), "r"(lo->y), "r"(lo->z),
-                                         "r"(lo->w), "r"(hi->x), "r"(hi->y), "r"(hi->z), "r"(hi->w) : "memory");
-                    } else {                           // turned over, so that W lanes write neighbouring outputs of a row
-                        __syncwarp();
-                        const uint32_t mine = smem_u32(scratch[ew]);
-                        sts128(mine + lane * 32, lo->x, lo->y, lo->z, lo->w);
-                        sts128(mine + lane * 32 + 16, hi->x, hi->y, hi->z, hi->w);
-                        __syncwarp();
-                        const T* turned = reinterpret_cast<const T*>(scratch[ew]);
+                    for (int q = 0; q < 8; q++) {
+                        alignas(16) T o[W / 8];
 #pragma unroll
-                        for (int q = 0; q < W; q++) {
-                            const int r = q * (32 / W) + lane / W, e = lane % W;
-                            if (m0 + r < p.M && e < left) static_cast<T*>(p.c)[(m0 + r) * p.ldc + n0 + h + e] = turned[r * W + e];
+                        for (int e = 0; e < W / 8; e++) o[e] = from_f32<T>(sum_of(h + q * (W / 8) + e));
+                        const uint4 u = *reinterpret_cast<const uint4*>(o);
+                        sts128(out + lane * 128 + ((q ^ (lane & 7)) << 4), u.x, u.y, u.z, u.w);
+                    }
+                    if (p.tma_out) {
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0 && n0 + h < p.N && m0 < p.M) {   // what lies outside c is not written
+                            asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];"
+                                         ::"l"(reinterpret_cast<uint64_t>(&out_map)), "r"((n0 + h) * (int)sizeof(T)), "r"(m0), "r"(out) : "memory");
+                            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                         }
+                    } else {                           // a row at a time, its outputs side by side
+                        __syncwarp();
+#pragma unroll 4
+                        for (int r = 0; r < 32; r++) {
+                            if (m0 + r >= p.M) break;
+#pragma unroll
+                            for (int e = lane; e < W; e += 32) {
+                                const uint32_t at = out + r * 128 + (((e * (int)sizeof(T) >> 4) ^ (r & 7)) << 4) + (e * (int)sizeof(T) & 15);
+                                T v;
+                                if constexpr (sizeof(T) == 4) v = lds_f32(at);
+                                else asm volatile("ld.shared.b16 %0, [%1];" : "=h"(reinterpret_cast<unsigned short&>(v)) : "r"(at));
+                                if (n0 + h + e < p.N) static_cast<T*>(p.c)[(long long)(m0 + r) * p.ldc + n0 + h + e] = v;
+                            }
+                        }
+                        __syncwarp();
                     }
                 }
             }
         }
+        if (!Cfg::FEW) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");   // the stores are complete before the CTA winds down
     }
 
     if (SPLIT) {
