@@ -161,6 +161,7 @@ __global__ void __launch_bounds__(Fp8Cfg<NT>::THREADS, Fp8Cfg<NT>::CTAS_PER_SM)
         }
     }
     if (threadIdx.x == 0) {
+        if (!Cfg::FEW && p.tma_out) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&out_map)));
         for (int i = 0; i < Cfg::STAGES; i++) { mbar_init(&bar_full[i], 1); mbar_init(&bar_empty[i], 1); }
         for (int i = 0; i < F8_GROUPS; i++) { mbar_init(&bar_factor_full[i], 1); mbar_init(&bar_factor_empty[i], Cfg::EPI_WARPS); }
         for (int i = 0; i < 2; i++) { mbar_init(&bar_acc_full[i], 1); mbar_init(&bar_acc_empty[i], (PAIR ? 2 : 1) * Cfg::EPI_WARPS); }
@@ -288,6 +289,8 @@ __global__ void __launch_bounds__(Fp8Cfg<NT>::THREADS, Fp8Cfg<NT>::CTAS_PER_SM)
                        factor_empty = smem_u32(bar_factor_empty);
         const uint32_t my_factors = smem_u32(factors) + (Cfg::FEW ? col0 : (col0 & ~127) + quarter * 32 + lane) * 4;
         bool ok = true;
+        int tm = first / p.tiles_n, tn = first - tm * p.tiles_n;
+        const int step_m = step / p.tiles_n, step_n = step - step_m * p.tiles_n;
         for (int tile = first; tile < p.ntiles && ok; tile += step) {
             float2 sum[Cfg::COLS / 2];
 #pragma unroll
@@ -346,9 +349,10 @@ __global__ void __launch_bounds__(Fp8Cfg<NT>::THREADS, Fp8Cfg<NT>::CTAS_PER_SM)
                 if (!acc) acc_par ^= 1;
             }
             if (!ok) break;
-            const int tm = tile / p.tiles_n, tn = tile - tm * p.tiles_n;
             const int m0 = Cfg::FEW ? tm * NT + col0 : (PAIR ? tm * 2 + rank : tm) * 128 + quarter * 32;   // first activation row and output of the warp
             const int n0 = Cfg::FEW ? tn * 128 + quarter * 32 : tn * NT + col0;
+            tm += step_m;                              // the next tile's place
+            if ((tn += step_n) >= p.tiles_n) { tn -= p.tiles_n; tm++; }
             if (SPLIT) {
                 // this CTA's part -> its shared memory (the ring is idle: its last loads have been multiplied), [column][output]
                 const uint32_t part = stage0 + (uint32_t)((col0 * 128 + quarter * 32 + lane) * 4);
