@@ -184,16 +184,21 @@ __global__ void __launch_bounds__(256) fp8_quantize_blocks_kernel(const T* __res
 static bool aligned_to(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
 // -------------------------------------------------------------------------------------------------
-// The product: which tile (its columns: 16, 32, 64 activation rows or 128, 256 weight rows), how many CTAs share one.
+// The product: which tile (its columns: 16, 32, 64 activation rows or 128, 256 weight rows).  Tiles of 128 rows where they
+// occupy half of the SMs (512 x 4096 x 4096: 13.9 us, 17.7 in columns of 64), pairs of CTAs on 256 x 256 where those do.
 static int f8_columns(int m, int n) {
     if (m <= 16) return 16;
     if (m <= 32) return 32;
-    if (m <= 64 || ((long long)m + 127) / 128 * ((n + 127) / 128) < sm_count()) return 64;
+    if (m <= 64 || ((long long)m + 127) / 128 * ((n + 127) / 128) < sm_count() / 2) return 64;
     return ((long long)m + 255) / 256 * ((n + 255) / 256) < sm_count() / 2 ? 128 : 256;
 }
+// How many CTAs share a tile: as many as find room, two to an SM, with four blocks of K or more each.  Joining their parts takes
+// 2 us, what a CTA needs for about eight blocks: 8 x 1024 x 4096 4.5 us (10.7 undivided), 1 x 8192 x 4096 9.2 (13.0), 256 x 2048
+// x 1024, of eight blocks, 7.5 divided and 5.6 undivided.
 static int f8_splits(long long ntiles, int nkb) {
     int s = 1;
-    while (s < F8_MAX_SPLIT && 2 * s * ntiles <= 2 * sm_count() && 4 * s <= nkb) s *= 2;
+    if (nkb >= 12)
+        while (s < F8_MAX_SPLIT && 2 * s * ntiles <= 2 * sm_count() && 8 * s <= nkb) s *= 2;
     return s;
 }
 

@@ -120,9 +120,9 @@ __device__ __forceinline__ void f8_fma2(float2& sum, uint32_t a, uint32_t b, flo
         "fma.rn.f32x2 s, v, c, s;\n\tmov.b64 {%0, %1}, s;\n\t}" : "+f"(sum.x), "+f"(sum.y) : "r"(a), "r"(b), "f"(sx), "f"(sy));
 }
 __device__ __forceinline__ void f8_tmem_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ float f8_ld_cluster(uint32_t addr, int rank) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(f8_in_cta(addr, rank)) : "memory");
+__device__ __forceinline__ float4 f8_ld_cluster(uint32_t addr, int rank) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(f8_in_cta(addr, rank)) : "memory");
     return v;
 }
 __device__ __forceinline__ void f8_cluster_sync() {
@@ -440,17 +440,23 @@ __global__ void __launch_bounds__(Fp8Cfg<NT>::THREADS, Fp8Cfg<NT>::CTAS_PER_SM)
         __syncwarp();
         f8_cluster_sync();
         const int tile = first, tm = tile / p.tiles_n, tn = tile - tm * p.tiles_n;
-        const int total = min(NT, p.M - tm * NT) * 128;
+        const int total = min(NT, p.M - tm * NT) * 32;   // in fours, whose trip over the cluster is what this takes
         const int lo = (int)((long long)total * rank / splits), hi = (int)((long long)total * (rank + 1) / splits);
         for (int idx = lo + (int)threadIdx.x; idx < hi; idx += Cfg::THREADS) {
-            float part[F8_MAX_SPLIT];
+            float4 part[F8_MAX_SPLIT];
 #pragma unroll
-            for (int r = 0; r < F8_MAX_SPLIT; r++) part[r] = r < splits ? f8_ld_cluster(stage0 + idx * 4, r) : 0.f;
-            float v = part[0];
+            for (int r = 0; r < F8_MAX_SPLIT; r++)
+                if (r < splits) part[r] = f8_ld_cluster(stage0 + idx * 16, r);
+            float4 v = part[0];
 #pragma unroll
-            for (int r = 1; r < F8_MAX_SPLIT; r++) v += part[r];
-            const int m = tm * NT + (idx >> 7), n = tn * 128 + (idx & 127);
-            if (n < p.N) static_cast<T*>(p.c)[m * p.ldc + n] = from_f32<T>(v + (p.bias ? __ldg(p.bias + n) : 0.f));
+            for (int r = 1; r < F8_MAX_SPLIT; r++)
+                if (r < splits) { v.x += part[r].x; v.y += part[r].y; v.z += part[r].z; v.w += part[r].w; }
+            const int m = tm * NT + (idx >> 5), n = tn * 128 + (idx & 31) * 4;
+            T* const out = static_cast<T*>(p.c) + m * p.ldc + n;
+            const float o[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (n + e < p.N) out[e] = from_f32<T>(o[e] + (p.bias ? __ldg(p.bias + n + e) : 0.f));
         }
         f8_cluster_sync();                             // no CTA leaves while its part is being read
     }

@@ -323,10 +323,14 @@ def _rows(t, what):
     if t.dim() == 2:
         rows, cols = t.shape
         if cols <= 1 or t.stride(1) == 1:
+            if rows >= 1 << 31 or cols >= 1 << 31:
+                raise ValueError(f"{what}: too large a matrix")
             return rows, cols, t.stride(0) if rows > 1 else cols
     elif t.dim() >= 1 and t.is_contiguous():
-        cols = t.shape[-1]
-        return (t.numel() // cols if cols else t.shape[:-1].numel()), cols, cols
+        rows, cols = t.shape[:-1].numel(), t.shape[-1]
+        if rows >= 1 << 31 or cols >= 1 << 31:
+            raise ValueError(f"{what}: too large a matrix")
+        return rows, cols, cols
     raise TypeError(f"{what}: expected a matrix with unit stride along its rows, or a contiguous tensor")
 
 
