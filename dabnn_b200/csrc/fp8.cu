@@ -184,13 +184,16 @@ __global__ void __launch_bounds__(256) fp8_quantize_blocks_kernel(const T* __res
 static bool aligned_to(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
 // -------------------------------------------------------------------------------------------------
-// The product: which tile (its columns: 16, 32, 64 activation rows or 128, 256 weight rows).  Tiles of 128 rows where they
-// occupy half of the SMs (512 x 4096 x 4096: 13.9 us, 17.7 in columns of 64), pairs of CTAs on 256 x 256 where those do.
+// The product: which tile (its columns: 16, 32, 64 activation rows or 128, 256 weight rows).  More than 64 rows have tiles of
+// 128 x 128 (512 x 4096 x 4096: 13.8 us, 17.5 in columns of 64), unless those are too few for a quarter of the SMs and K is
+// better divided (100 x 1000 x 4096: 7.1 us in columns of 64, 13 in eight tiles of 128), or more than one for an SM: then pairs
+// of CTAs have 256 x 256 (2048 x 2048 x 2048: 12.7 us, 14.7 in tiles of 128; 1024 x 1024 x 4096, 64 tiles: 17.3 and 13.1).
 static int f8_columns(int m, int n) {
     if (m <= 16) return 16;
     if (m <= 32) return 32;
-    if (m <= 64 || ((long long)m + 127) / 128 * ((n + 127) / 128) < sm_count() / 2) return 64;
-    return ((long long)m + 255) / 256 * ((n + 255) / 256) < sm_count() / 2 ? 128 : 256;
+    const long long tiles = ((long long)m + 127) / 128 * ((n + 127) / 128);
+    if (m <= 64 || 4 * tiles < sm_count()) return 64;
+    return tiles <= sm_count() ? 128 : 256;
 }
 // How many CTAs share a tile: as many as find room, two to an SM, with four blocks of K or more each.  Joining their parts takes
 // 2 us, what a CTA needs for about eight blocks: 8 x 1024 x 4096 4.5 us (10.7 undivided), 1 x 8192 x 4096 9.2 (13.0), 256 x 2048
