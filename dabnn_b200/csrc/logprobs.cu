@@ -318,6 +318,10 @@ __device__ __forceinline__ void lp_scan(const LogprobsParams& p, const T* row, i
     if (TEAM && ENTRIES && part >= batches) team_sync();   // nothing to do but to let the others pass
     for (int b = part; b < batches; b += parts) {
         if (b != part) load(b);
+        {   // the next batch on its way to L2 (one ahead: 2048 rows of 32768 fp32 67 us, 71 without, four ahead 71)
+            const long long next = (long long)(b + parts) * BATCH - shift + lane * (128 / (int)sizeof(T));
+            if (lane < VECS * 4 && next >= 0 && next < n) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + next));
+        }
         const float half[2] = {vec_max(v[0], v[1]), vec_max(v[2], v[3])};
         const float top = max_nan(half[0], half[1]);
         const float to = fmaxf(all.m, top);        // (a NaN is passed over: it makes S one)
