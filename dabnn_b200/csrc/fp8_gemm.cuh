@@ -47,7 +47,7 @@ struct Fp8Cfg {                                        // NT: columns of a tile
     static constexpr int EPI_WARPS = FEW ? 4 : NT / 16;
     static constexpr int EPI_WARP0 = PAIR ? 4 : 3, THREADS = (EPI_WARP0 + EPI_WARPS) * 32;
     static constexpr int COLS = NT / (EPI_WARPS / 4);  // accumulator columns of an epilogue warp
-    static constexpr int FACTORS = NT;      // of a block: one per column / per lane and 128 columns
+    static constexpr int FACTORS = NT;                 // of a block: one per column / per lane and 128 columns
     static constexpr int COL_ROWS = PAIR ? NT / 2 : NT;  // rows of the column operand that a CTA loads
     static constexpr int STAGE_BYTES = F8_L_BYTES + COL_ROWS * F8_BLOCK;
     static constexpr int STAGES = NT <= 32 ? 5 : NT == 64 ? 4 : NT == 128 ? 5 : 4;
@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(Fp8Cfg<NT>::THREADS, Fp8Cfg<NT>::CTAS_PER_SM)
     __shared__ __align__(8) uint64_t bar_factor_full[F8_GROUPS], bar_factor_empty[F8_GROUPS];
     __shared__ __align__(16) float factors[F8_GROUPS][F8_GROUP][Cfg::FACTORS];
     __shared__ uint32_t tmem_base_s;
-    __shared__ int s_abort;
+    __shared__ int s_abort, s_loads;
 
     const int warp = uniform_warp(), lane = threadIdx.x & 31;
     const uint32_t stage0 = (smem_u32(smem_dyn) + 1023u) & ~1023u;
@@ -167,117 +167,120 @@ __global__ void __launch_bounds__(Fp8Cfg<NT>::THREADS, Fp8Cfg<NT>::CTAS_PER_SM)
         for (int i = 0; i < 2; i++) { mbar_init(&bar_acc_full[i], 1); mbar_init(&bar_acc_empty[i], (PAIR ? 2 : 1) * Cfg::EPI_WARPS); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::);
         s_abort = 0;
+        s_loads = 0;
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     if (PAIR) f8_cluster_sync();                       // the other CTA's barriers are set up
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem_base = tmem_base_s;
-    grid_launch_dependents();
+    // In this order: a kernel that this lets start may read its constants at once, and they may come from a launch before this one.
     grid_dependency_wait();
+    grid_launch_dependents();
     if (warp < Cfg::EPI_WARP0) {
-    // a pair's 20 warps have 96 registers each at launch: these four give 32 of theirs to the epilogue's sixteen, whose sums and two
-    // chunks of an accumulator take 96
-    if (PAIR) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-    if (warp == 0) {
-        // =========================== TMA loads: one lane ===========================
-        if (elect_lane()) {
-            uint32_t s = 0, use = 0;
-            bool ok = true;
-            for (int tile = first; tile < p.ntiles && ok; tile += step) {
-                const int tm = tile / p.tiles_n, tn = tile - tm * p.tiles_n;
-                for (int kb = kb0; kb < kb1; kb++) {
-                    if (use >= 1 && !mbar_wait(&bar_empty[s], (use - 1) & 1, abort_flag)) {
-                        atomicCAS(&g_fp8_status, 0, 51);
+        // a pair's 20 warps have 96 registers each at launch: these four give 32 of theirs to the epilogue's sixteen, whose sums and two
+        // chunks of an accumulator take 96
+        if (PAIR) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        if (warp == 0) {
+            // =========================== TMA loads: one lane ===========================
+            if (elect_lane()) {
+                uint32_t s = 0, use = 0;
+                bool ok = true;
+                for (int tile = first; tile < p.ntiles && ok; tile += step) {
+                    const int tm = tile / p.tiles_n, tn = tile - tm * p.tiles_n;
+                    for (int kb = kb0; kb < kb1; kb++) {
+                        if (use >= 1 && !mbar_wait(&bar_empty[s], (use - 1) & 1, abort_flag)) {
+                            atomicCAS(&g_fp8_status, 0, 51);
+                            s_abort = 1;
+                            ok = false;
+                            break;
+                        }
+                        const uint32_t at = stage0 + s * Cfg::STAGE_BYTES;
+                        uint32_t bar = smem_u32(&bar_full[s]);
+                        if (!PAIR || rank == 0)
+                            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"((PAIR ? 2 : 1) * Cfg::STAGE_BYTES) : "memory");
+                        if (PAIR) bar = f8_in_cta(bar, 0);   // the CTA that issues for both waits for both
+                        f8_load<PAIR>(at, &lane_map, kb * F8_BLOCK, (Cfg::FEW ? tn : PAIR ? tm * 2 + rank : tm) * 128, bar);
+                        f8_load<PAIR>(at + F8_L_BYTES, &col_map, kb * F8_BLOCK, (Cfg::FEW ? tm : tn) * NT + (PAIR ? rank * Cfg::COL_ROWS : 0), bar);
+                        if (++s == Cfg::STAGES) { s = 0; use++; }
+                    }
+                }
+                s_loads = (int)(use * Cfg::STAGES + s);
+            }
+        } else if (warp == 1) {
+            // =========================== MMA issue: the whole warp walks, one lane issues, for a pair the first CTA's ===========================
+            const bool leader = elect_lane();
+            constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(NT >> 3) << 17) | ((uint32_t)((PAIR ? 256 : 128) >> 4) << 24);   // D f32, A = B = e4m3, K-major
+            uint32_t s = 0, par = 0;
+            bool ok = !PAIR || rank == 0;
+            int i = 0;   // blocks so far
+            for (int tile = first; tile < p.ntiles && ok; tile += step)
+                for (int kb = kb0; kb < kb1; kb++, i++) {
+                    const int acc = i & 1;
+                    if (i >= 2 && !f8_wait(smem_u32(&bar_acc_empty[acc]), ((i >> 1) - 1) & 1, abort_flag)) {
+                        atomicCAS(&g_fp8_status, 0, 52);
                         s_abort = 1;
                         ok = false;
                         break;
                     }
-                    const uint32_t at = stage0 + s * Cfg::STAGE_BYTES;
-                    uint32_t bar = smem_u32(&bar_full[s]);
-                    if (!PAIR || rank == 0)
-                        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"((PAIR ? 2 : 1) * Cfg::STAGE_BYTES) : "memory");
-                    if (PAIR) bar = f8_in_cta(bar, 0);   // the CTA that issues for both waits for both
-                    f8_load<PAIR>(at, &lane_map, kb * F8_BLOCK, (Cfg::FEW ? tn : PAIR ? tm * 2 + rank : tm) * 128, bar);
-                    f8_load<PAIR>(at + F8_L_BYTES, &col_map, kb * F8_BLOCK, (Cfg::FEW ? tm : tn) * NT + (PAIR ? rank * Cfg::COL_ROWS : 0), bar);
-                    if (++s == Cfg::STAGES) { s = 0; use++; }
+                    if (!f8_wait(smem_u32(&bar_full[s]), par, abort_flag)) {
+                        atomicCAS(&g_fp8_status, 0, 53);
+                        s_abort = 1;
+                        ok = false;
+                        break;
+                    }
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint64_t l = f8_desc(stage0 + s * Cfg::STAGE_BYTES), c = l + (F8_L_BYTES >> 4);
+                    if (leader) {
+#pragma unroll
+                        for (int j = 0; j < F8_BLOCK / 32; j++) f8_mma<PAIR>(tmem_base + acc * NT, l + 2 * j, c + 2 * j, idesc, j > 0);
+                        f8_commit<PAIR>(smem_u32(&bar_empty[s]));
+                        f8_commit<PAIR>(smem_u32(&bar_acc_full[acc]));
+                    }
+                    __syncwarp();
+                    if (++s == Cfg::STAGES) { s = 0; par ^= 1u; }
+                }
+        } else if (warp == 2) {
+            // =========================== factors as * bs ===========================
+            // FEW: a lane has the columns lane, lane + 32; else rows lane + 32 j of the tile, each with the bs of every 128 columns
+            constexpr int MINE = Cfg::FEW ? (NT + 31) / 32 : 4, BLOCKS = Cfg::FEW ? 1 : NT / 128;
+            int i = 0;
+            bool ok = true;
+            for (int tile = first; tile < p.ntiles && ok; tile += step) {
+                const int tm = tile / p.tiles_n, tn = tile - tm * p.tiles_n;
+                const int m0 = (Cfg::FEW ? tm * NT : (PAIR ? tm * 2 + rank : tm) * 128) + lane;
+                const float* a = p.as + m0 * p.as_row + kb0 * p.as_block;
+                const float* b = p.bs + (long long)tn * BLOCKS * p.bs_row + kb0 * p.bs_block;
+                for (int kb = kb0; kb < kb1; kb += F8_GROUP, i++) {   // (a tile begins with a new group)
+                    float av[F8_GROUP][MINE], bv[F8_GROUP][BLOCKS];
+#pragma unroll
+                    for (int g = 0; g < F8_GROUP; g++) {
+#pragma unroll
+                        for (int e = 0; e < MINE; e++) av[g][e] = kb + g < kb1 && m0 + e * 32 < p.M ? __ldg(a + e * 32 * p.as_row) : 0.f;
+#pragma unroll
+                        for (int e = 0; e < BLOCKS; e++) bv[g][e] = kb + g < kb1 && (tn * BLOCKS + e) * 128 < p.N ? __ldg(b + e * p.bs_row) : 0.f;
+                        a += p.as_block;
+                        b += p.bs_block;
+                    }
+                    const int slot = i % F8_GROUPS;
+                    if (i >= F8_GROUPS && !f8_wait(smem_u32(&bar_factor_empty[slot]), (i / F8_GROUPS - 1) & 1, abort_flag)) {
+                        atomicCAS(&g_fp8_status, 0, 55);
+                        s_abort = 1;
+                        ok = false;
+                        break;
+                    }
+#pragma unroll
+                    for (int g = 0; g < F8_GROUP; g++)
+#pragma unroll
+                        for (int e = 0; e < MINE; e++)
+#pragma unroll
+                            for (int h = 0; h < BLOCKS; h++)
+                                if (!Cfg::FEW || e * 32 + lane < NT) factors[slot][g][h * 128 + e * 32 + lane] = av[g][e] * bv[g][h];
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&bar_factor_full[slot]);
                 }
             }
         }
-    } else if (warp == 1) {
-        // =========================== MMA issue: the whole warp walks, one lane issues, for a pair the first CTA's ===========================
-        const bool leader = elect_lane();
-        constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(NT >> 3) << 17) | ((uint32_t)((PAIR ? 256 : 128) >> 4) << 24);   // D f32, A = B = e4m3, K-major
-        uint32_t s = 0, par = 0;
-        bool ok = !PAIR || rank == 0;
-        int i = 0;   // blocks so far
-        for (int tile = first; tile < p.ntiles && ok; tile += step)
-            for (int kb = kb0; kb < kb1; kb++, i++) {
-                const int acc = i & 1;
-                if (i >= 2 && !f8_wait(smem_u32(&bar_acc_empty[acc]), ((i >> 1) - 1) & 1, abort_flag)) {
-                    atomicCAS(&g_fp8_status, 0, 52);
-                    s_abort = 1;
-                    ok = false;
-                    break;
-                }
-                if (!f8_wait(smem_u32(&bar_full[s]), par, abort_flag)) {
-                    atomicCAS(&g_fp8_status, 0, 53);
-                    s_abort = 1;
-                    ok = false;
-                    break;
-                }
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint64_t l = f8_desc(stage0 + s * Cfg::STAGE_BYTES), c = l + (F8_L_BYTES >> 4);
-                if (leader) {
-#pragma unroll
-                    for (int j = 0; j < F8_BLOCK / 32; j++) f8_mma<PAIR>(tmem_base + acc * NT, l + 2 * j, c + 2 * j, idesc, j > 0);
-                    f8_commit<PAIR>(smem_u32(&bar_empty[s]));
-                    f8_commit<PAIR>(smem_u32(&bar_acc_full[acc]));
-                }
-                __syncwarp();
-                if (++s == Cfg::STAGES) { s = 0; par ^= 1u; }
-            }
-    } else if (warp == 2) {
-        // =========================== factors as * bs ===========================
-        // FEW: a lane has the columns lane, lane + 32; else rows lane + 32 j of the tile, each with the bs of every 128 columns
-        constexpr int MINE = Cfg::FEW ? (NT + 31) / 32 : 4, BLOCKS = Cfg::FEW ? 1 : NT / 128;
-        int i = 0;
-        bool ok = true;
-        for (int tile = first; tile < p.ntiles && ok; tile += step) {
-            const int tm = tile / p.tiles_n, tn = tile - tm * p.tiles_n;
-            const int m0 = (Cfg::FEW ? tm * NT : (PAIR ? tm * 2 + rank : tm) * 128) + lane;
-            const float* a = p.as + m0 * p.as_row + kb0 * p.as_block;
-            const float* b = p.bs + (long long)tn * BLOCKS * p.bs_row + kb0 * p.bs_block;
-            for (int kb = kb0; kb < kb1; kb += F8_GROUP, i++) {   // (a tile begins with a new group)
-                float av[F8_GROUP][MINE], bv[F8_GROUP][BLOCKS];
-#pragma unroll
-                for (int g = 0; g < F8_GROUP; g++) {
-#pragma unroll
-                    for (int e = 0; e < MINE; e++) av[g][e] = kb + g < kb1 && m0 + e * 32 < p.M ? __ldg(a + e * 32 * p.as_row) : 0.f;
-#pragma unroll
-                    for (int e = 0; e < BLOCKS; e++) bv[g][e] = kb + g < kb1 && (tn * BLOCKS + e) * 128 < p.N ? __ldg(b + e * p.bs_row) : 0.f;
-                    a += p.as_block;
-                    b += p.bs_block;
-                }
-                const int slot = i % F8_GROUPS;
-                if (i >= F8_GROUPS && !f8_wait(smem_u32(&bar_factor_empty[slot]), (i / F8_GROUPS - 1) & 1, abort_flag)) {
-                    atomicCAS(&g_fp8_status, 0, 55);
-                    s_abort = 1;
-                    ok = false;
-                    break;
-                }
-#pragma unroll
-                for (int g = 0; g < F8_GROUP; g++)
-#pragma unroll
-                    for (int e = 0; e < MINE; e++)
-#pragma unroll
-                        for (int h = 0; h < BLOCKS; h++)
-                            if (!Cfg::FEW || e * 32 + lane < NT) factors[slot][g][h * 128 + e * 32 + lane] = av[g][e] * bv[g][h];
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&bar_factor_full[slot]);
-            }
-        }
-    }
     } else {
         // =========================== epilogue ===========================
         if (PAIR) asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
@@ -458,10 +461,16 @@ __global__ void __launch_bounds__(Fp8Cfg<NT>::THREADS, Fp8Cfg<NT>::CTAS_PER_SM)
             for (int e = 0; e < 4; e++)
                 if (n + e < p.N) out[e] = from_f32<T>(o[e] + (p.bias ? __ldg(p.bias + n + e) : 0.f));
         }
+        __syncwarp();
         f8_cluster_sync();                             // no CTA leaves while its part is being read
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    if (s_abort && (!PAIR || rank == 0) && threadIdx.x == 0) {   // loads may be on their way still (a pair's all arrive at the first CTA's barriers)
+        const int never = 0;
+        for (int i = max(0, s_loads - Cfg::STAGES); i < s_loads; i++) mbar_wait(&bar_full[i % Cfg::STAGES], (i / Cfg::STAGES) & 1, &never);
+    }
+    __syncwarp();
     if (PAIR) f8_cluster_sync();                       // no CTA leaves while the other arrives at its barriers
     if (warp == 1) {
         __syncwarp();

@@ -277,6 +277,77 @@ def test_gemm_leading_dimensions_streams_and_graphs(ops):
         assert torch.equal(graphs[i][1], expected)
 
 
+@pytest.mark.parametrize("m,n,k", [(5, 300, 2048), (100, 520, 512), (1000, 2600, 384)])
+def test_gemm_scales_without_a_number(ops, m, n, k):
+    """A scale that is NaN or infinite reaches the outputs of its row, or of its 128 columns, and no other."""
+    a, sa, b, sb, bias = operands(m, n, k, 12, powers=True)
+    c, tol = R.gemm(a, sa, b, sb, bias, torch.finfo(torch.float32).eps)
+    da, db = dev(sa), dev(sb)
+    da[m - 1, k // 128 - 1] = float("nan")
+    db[1, 0] = float("nan")
+    got = values(ops.fp8_gemm(R.f8(a), da, R.f8(b), db, dev(bias)))
+    expected = c.copy()
+    expected[m - 1] = np.nan
+    expected[:, 128:256] = np.nan
+    R.close(got, expected, tol)
+
+
+@pytest.mark.parametrize("m", [4, 200, 3000])
+def test_launches_one_after_the_other(ops, m):
+    """Each call of a chain reads what the call before wrote, in memory that the allocator hands round, with nothing in between:
+    the same bits as with a synchronisation after every call."""
+    g = torch.Generator().manual_seed(m)
+    w = [(torch.randn((384, 384), generator=g) * 384 ** -0.5).cuda() for _ in range(3)]
+    x0 = torch.randn((m, 384), generator=g).cuda()
+
+    def chain(wait):
+        x, out = x0.clone(), []
+        for i in range(24):
+            wq, ws = ops.fp8_quantize_weights(w[i % 3])
+            q, s = ops.fp8_quantize(x)
+            x = ops.fp8_gemm(q, s, wq, ws)
+            out.append(ops.logprobs(x, None, 3)[4])
+            if wait:
+                torch.cuda.synchronize()
+        return x, torch.stack(out)
+
+    for a, b in zip(chain(True), chain(False)):
+        assert torch.equal(a, b)
+
+
+def test_two_streams_at_once(ops):
+    """Calls of every shape side by side: they share no memory."""
+    shapes = [(1, 2000, 4096), (40, 1000, 2048), (300, 1500, 768), (1500, 2600, 512)]
+    sets = []
+    for m, n, k in shapes:
+        a, sa, b, sb, bias = operands(m, n, k, m)
+        args = (R.f8(a), dev(sa), R.f8(b), dev(sb), dev(bias))
+        sets.append((args, ops.fp8_gemm(*args)))
+    torch.cuda.synchronize()
+    streams, results = [torch.cuda.Stream() for _ in range(2)], []
+    for round_ in range(6):
+        for j, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                for i in range(len(sets)):
+                    args, expected = sets[(i + j * 2 + round_) % len(sets)]
+                    results.append((ops.fp8_gemm(*args), expected))
+    torch.cuda.synchronize()
+    for got, expected in results:
+        assert torch.equal(got, expected)
+
+
+def test_a_wait_that_gave_up_is_reported(ops):
+    """The code is planted from the host; no kernel is made to stall."""
+    from dabnn_b200 import capi
+    lib = capi.load()
+    assert ops.engine_status() == 0
+    capi.check(lib.dabnn_debug_raise_engine_status(3, 54))
+    assert ops.engine_status() == 54
+    capi.check(lib.dabnn_debug_raise_engine_status(3, 0))
+    assert ops.engine_status() == 0
+    assert lib.dabnn_debug_raise_engine_status(4, 1) == 1
+
+
 # ---------------------------------------------------------------------------------------------- the head as a whole
 @pytest.mark.parametrize("m,classes,k", [(1, 1000, 512), (64, 1000, 512), (200, 365, 1100)])
 def test_classifier_head(ops, m, classes, k):

@@ -64,6 +64,33 @@ def test_logprobs_many_rows(ops):
     check(ops, x, labels, 5)
 
 
+@pytest.mark.parametrize("kind,classes,top", [("bf16", 4500, 8), ("f32", 4200, 0), ("f16", 4301, 40)])
+def test_logprobs_many_wide_rows(ops, kind, classes, top):
+    """Enough rows for a warp each."""
+    x, labels = rows_of(3700, classes, 5, kind)
+    check(ops, x, labels, top)
+
+
+def test_two_streams_at_once(ops):
+    sets = []
+    for rows, classes, top in ((1, 100000, 20), (700, 1000, 5), (3, 30000, 64), (150, 9000, 8)):
+        x, labels = rows_of(rows, classes, rows, "bf16")
+        lab = torch.tensor(labels).cuda()
+        sets.append((x, lab, top, ops.logprobs(x, lab, top)))
+    torch.cuda.synchronize()
+    streams, results = [torch.cuda.Stream() for _ in range(2)], []
+    for round_ in range(6):
+        for j, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                for i in range(len(sets)):
+                    x, lab, top, expected = sets[(i + j * 2 + round_) % len(sets)]
+                    results.append((ops.logprobs(x, lab, top), expected))
+    torch.cuda.synchronize()
+    for got, expected in results:
+        for a, b in zip(got, expected):
+            assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("classes", [70, 1000, 9000, 40000])
 @pytest.mark.parametrize("kind", TYPES)
 def test_ties_and_orders(ops, classes, kind):
