@@ -341,7 +341,9 @@ __device__ __forceinline__ void lp_scan(const LogprobsParams& p, const T* row, i
         all.s += s.x + s.y;
         all.w += w.x + w.y;
 
-        if (have) {
+        // nothing of most batches comes before a label that is among the likeliest (4096 rows of 65536 bf16, top 8: 123 us with the
+        // likeliest classes as labels, 139 with any)
+        if (have && __any_sync(0xffffffffu, !(top < mine))) {
             Count<T> c;
 #pragma unroll
             for (int i = 0; i < VECS; i++) c.add(v[i], first + i * 32 * N + N <= label ? many_front : many_behind);
