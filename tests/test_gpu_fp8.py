@@ -169,7 +169,7 @@ def test_gemm_large(ops):
 
 @pytest.mark.parametrize("out", TYPES)
 @pytest.mark.parametrize("bias", [False, True])
-@pytest.mark.parametrize("m,n,k", [(1, 1000, 512), (20, 131, 300), (150, 259, 384), (300, 1001, 200)])
+@pytest.mark.parametrize("m,n,k", [(1, 1000, 512), (20, 131, 300), (150, 259, 384), (300, 1001, 200), (700, 1304, 200), (700, 1301, 200), (2300, 2104, 300), (1900, 2101, 300)])
 def test_gemm_output_types(ops, m, n, k, out, bias):
     check_gemm(ops, m, n, k, out, bias)
 
