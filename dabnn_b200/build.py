@@ -15,7 +15,7 @@ CSRC = HERE / "csrc"
 LIB = HERE / "lib" / "libdabnn_b200.so"
 SOURCES = ["api.cu", "bitpack.cu", "float_layers.cu", "contraction.cu", "bconv_u8.cu", "net.cu", "peaks.cu", "binconv_static.cu", "fp8.cu", "logprobs.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
-              "-Xcompiler", "-fPIC", "-shared", "--cudart=static"]
+              "-Xcompiler", "-fPIC", "-shared", "--cudart=static", "--threads", "0"]   # (0: a source on each core)
 
 
 def sources():
