@@ -344,21 +344,36 @@ __device__ __forceinline__ void lp_scan(const LogprobsParams& p, const T* row, i
         // nothing of most batches comes before a label that is among the likeliest (4096 rows of 65536 bf16, top 8: 123 us with the
         // likeliest classes as labels, 139 with any)
         if (have && __any_sync(0xffffffffu, !(top < mine))) {
-            Count<T> c;
+            int count = 0;
+            auto pick = [&](int i) {                   // v[i], i not known to the compiler
+                Vec<T> u = v[0];
 #pragma unroll
-            for (int i = 0; i < VECS; i++) c.add(v[i], first + i * 32 * N + N <= label ? many_front : many_behind);
-            int count = c.total();
-            // the label's own vector, and labels whose thresholds are of no use: one by one
-            if (all_front || none_behind || (unsigned)(label - first) < (unsigned)((VECS - 1) * 32 * N + N)) {
+                for (int k = 1; k < VECS; k++)
+                    if (i == k) u = v[k];
+                return u;
+            };
+            if (!all_front && !none_behind) {
+                Count<T> c;
+#pragma unroll
+                for (int i = 0; i < VECS; i++) c.add(v[i], first + i * 32 * N + N <= label ? many_front : many_behind);
+                count = c.total();
+                const unsigned off = (unsigned)(label - first), at = off % (32 * N);
+                if (off < VECS * 32 * N && at < N) {   // the label's own vector: what equals it in front of it is still to be counted
+                    const Vec<T> u = pick(off / (32 * N));
+#pragma unroll
+                    for (int e = 0; e < N - 1; e++) count += e < (int)at && u.value(e) == mine;
+                }
+            } else {                                   // no threshold serves: one by one
                 const float thr_front = pass_from(order_key(mine)), thr_behind = pass_above(order_key(mine));
-                count = 0;
-#pragma unroll
-                for (int i = 0; i < VECS; i++)
+#pragma unroll 1
+                for (int i = 0; i < VECS; i++) {
+                    const Vec<T> u = pick(i);
 #pragma unroll
                     for (int e = 0; e < N; e++) {
                         const int at = first + i * 32 * N + e;
-                        if (at >= 0 && at < n && (at < label ? !all_front && !(v[i].value(e) <= thr_front) : at > label && !none_behind && !(v[i].value(e) <= thr_behind))) count++;
+                        if (at >= 0 && at < n && (at < label ? !all_front && !(u.value(e) <= thr_front) : at > label && !none_behind && !(u.value(e) <= thr_behind))) count++;
                     }
+                }
             }
             before += count;
         }
@@ -584,7 +599,8 @@ __global__ void __launch_bounds__(LP_WARPS * 32, 4) logprobs_team_kernel(const L
 
 // Rows of one batch have a warp each; so do those of up to 4096 classes where every scheduler finds a row, and all where there
 // are 24 rows for an SM (4096 rows of 65536 bf16, top 8: 137 us with a warp each, 195 with a CTA; 1024 rows: 53 with a CTA).
-// Others a CTA, or as many CTAs (up to 8) as keep the SMs busy and find a batch for each of their warps.
+// Others a CTA, or as many CTAs (up to 8) as keep the SMs busy and find a batch for each of their warps: no more than three to an
+// SM (100 rows of 50000 bf16: 14.2 us in four CTAs each, 15.7 in two, 22 in eight).
 template <typename T, int ENTRIES>
 static int lp_launch(const LogprobsParams& p, cudaStream_t stream) {
     if (p.classes <= 128 * Vec<T>::N || (p.classes <= 4096 && p.rows >= 4 * sm_count()) || p.rows >= 24 * sm_count()) {
@@ -592,7 +608,7 @@ static int lp_launch(const LogprobsParams& p, cudaStream_t stream) {
         return DABNN_OK;
     }
     int ctas = 1;
-    while (ctas < LP_MAX_CLUSTER && (long long)p.rows * ctas * 2 <= 2 * sm_count() && (long long)ctas * LP_WARPS * 128 * Vec<T>::N < p.classes) ctas *= 2;
+    while (ctas < LP_MAX_CLUSTER && (long long)p.rows * ctas * 2 <= 3 * sm_count() && (long long)ctas * LP_WARPS * 128 * Vec<T>::N < p.classes) ctas *= 2;
     DABNN_REQUIRE((long long)p.rows * ctas <= INT_MAX, DABNN_ERR_SHAPE, "logprobs: too many rows");
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(p.rows * ctas));
