@@ -292,9 +292,18 @@ __device__ __forceinline__ void lp_scan(const LogprobsParams& p, const T* row, i
             const uint4* const at = reinterpret_cast<const uint4*>(row + first);
 #pragma unroll
             for (int i = 0; i < VECS; i++) v[i].raw = __ldg(at + i * 32);
-        } else {
+        } else if constexpr (TEAM) {
 #pragma unroll
             for (int i = 0; i < VECS; i++) v[i].load(row, first + i * 32 * N, n);
+        } else {                                       // (less code: 4096 rows of 65536 bf16 124 us instead of 130, 1024 of 1000 fp32 6.2 instead of 5.6)
+#pragma unroll 1
+            for (int i = 0; i < VECS; i++) {
+                Vec<T> u;
+                u.load(row, first + i * 32 * N, n);
+#pragma unroll
+                for (int k = 0; k < VECS; k++)
+                    if (i == k) v[k] = u;
+            }
         }
     };
     load(part);
