@@ -350,8 +350,8 @@ __device__ __forceinline__ void lp_scan(const LogprobsParams& p, const T* row, i
         all.s += s.x + s.y;
         all.w += w.x + w.y;
 
-        // nothing of most batches comes before a label that is among the likeliest (4096 rows of 65536 bf16, top 8: 123 us with the
-        // likeliest classes as labels, 139 with any)
+        // nothing of most batches comes before a label that is among the likeliest (4096 rows of 65536 bf16, top 8: 113 us with the
+        // likeliest classes as labels, 127 with any)
         if (have && __any_sync(0xffffffffu, !(top < mine))) {
             int count = 0;
             auto pick = [&](int i) {                   // v[i], i not known to the compiler
@@ -607,12 +607,13 @@ __global__ void __launch_bounds__(LP_WARPS * 32, 4) logprobs_team_kernel(const L
 }
 
 // Rows of one batch have a warp each; so do those of up to 4096 classes where every scheduler finds a row, and all where there
-// are 24 rows for an SM (4096 rows of 65536 bf16, top 8: 137 us with a warp each, 195 with a CTA; 1024 rows: 53 with a CTA).
+// are 16 rows for an SM (of 65536 bf16, top 8: 4096 rows 124 us with a warp each and 150 with a CTA, 2600 rows 95 and 99, 1900
+// rows 85 and 74).
 // Others a CTA, or as many CTAs (up to 8) as keep the SMs busy and find a batch for each of their warps: no more than three to an
 // SM (100 rows of 50000 bf16: 14.2 us in four CTAs each, 15.7 in two, 22 in eight).
 template <typename T, int ENTRIES>
 static int lp_launch(const LogprobsParams& p, cudaStream_t stream) {
-    if (p.classes <= 128 * Vec<T>::N || (p.classes <= 4096 && p.rows >= 4 * sm_count()) || p.rows >= 24 * sm_count()) {
+    if (p.classes <= 128 * Vec<T>::N || (p.classes <= 4096 && p.rows >= 4 * sm_count()) || p.rows >= 16 * sm_count()) {
         DABNN_CUDA_OK(launch_overlapped(logprobs_warp_kernel<T, ENTRIES>, dim3((unsigned)(((long long)p.rows + LP_ROWS - 1) / LP_ROWS)), dim3(LP_ROWS * 32), 0, stream, p));
         return DABNN_OK;
     }

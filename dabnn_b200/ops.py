@@ -341,7 +341,7 @@ def _fp8_quantize(x, block_rows):
         raise TypeError("fp8_quantize: expected fp32, fp16 or bf16")
     rows, k, ld = _rows(x, "fp8_quantize")
     pitch, blocks = (k + 15) // 16 * 16, (k + FP8_BLOCK - 1) // FP8_BLOCK
-    q = torch.empty(rows, pitch, dtype=torch.float8_e4m3fn, device=x.device)   # (a shape of its own costs 0.7 us more)
+    q = torch.empty_strided((rows, k), (pitch, 1), dtype=torch.float8_e4m3fn, device=x.device)
     if block_rows == 1:   # block by block: the order in which the product reads them
         scales = torch.empty_strided((rows, blocks), (1, rows), dtype=torch.float32, device=x.device)
         step, block_step = 1, rows
@@ -349,7 +349,7 @@ def _fp8_quantize(x, block_rows):
         scales = torch.empty((rows + block_rows - 1) // block_rows, blocks, dtype=torch.float32, device=x.device)
         step, block_step = blocks, 1
     check(capi.load().dabnn_fp8_quantize(x.data_ptr(), kind, ld, q.data_ptr(), pitch, scales.data_ptr(), step, block_step, rows, k, block_rows, _stream()))
-    return (q if pitch == k else q[:, :k]), scales
+    return q, scales
 
 
 def fp8_quantize(x):

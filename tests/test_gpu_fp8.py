@@ -213,6 +213,34 @@ def test_gemm_strides(ops, m):
     assert (out == -5).all()
 
 
+@pytest.mark.parametrize("m", [2, 70, 900])
+def test_gemm_broadcast_scales(ops, m):
+    """One scale for everything, one for each row, one for each block of K: strides of zero."""
+    n, k = 1400, 300
+    a, _, b, _, _ = operands(m, n, k, 31)
+    row, block = np.arange(1.0, m + 1)[:, None] / 64, np.array([[0.5, -2.0, 3.0]])
+    for one in (np.full((1, 1), 0.25), row, block):
+        for other in (np.full((1, 1), 0.125), block):
+            c, tol = R.gemm(a, np.broadcast_to(one, (m, 3)), b, np.broadcast_to(other, (11, 3)), None, torch.finfo(torch.float32).eps)
+            R.close(values(ops.fp8_gemm(R.f8(a), dev(one).expand(m, 3), R.f8(b), dev(other).expand(11, 3))), c, tol)
+
+
+@pytest.mark.parametrize("m,n,pitch,ldc", [(3, 300, 1 << 31, (1 << 31) + 16), (130, 2500, 1 << 25, (1 << 25) + 4), (130, 2500, 1 << 25, (1 << 25) + 1)])
+def test_gemm_offsets_beyond_32_bits(ops, m, n, pitch, ldc):
+    """Rows of the activations and of the output that begin beyond 2^32 bytes and elements of their bases."""
+    from dabnn_b200 import capi
+    k = 272
+    a, sa, b, sb, bias = operands(m, n, k, 21)
+    c, tol = R.gemm(a, sa, b, sb, bias, torch.finfo(torch.float32).eps)
+    wide = torch.empty((m - 1) * pitch + k, dtype=torch.float8_e4m3fn, device="cuda").as_strided((m, k), (pitch, 1))
+    wide.copy_(R.f8(a))
+    s, t, q = dev(sa), dev(sb), R.f8(b)
+    out = torch.empty((m - 1) * ldc + n, device="cuda").as_strided((m, n), (ldc, 1))
+    capi.check(capi.load().dabnn_fp8_gemm(wide.data_ptr(), pitch, s.data_ptr(), *s.stride(), q.data_ptr(), q.stride(0), t.data_ptr(), *t.stride(),
+                                          dev(bias).data_ptr(), out.data_ptr(), 0, ldc, m, n, k, ops._stream()))
+    R.close(values(out), c, tol)
+
+
 @pytest.mark.parametrize("m,n", [(4, 300), (90, 300), (300, 300)])
 def test_gemm_special_values(ops, m, n):
     """NaN bytes reach the outputs of their row and column and no other; scales of zero; blocks of zeros."""
