@@ -14,7 +14,8 @@ namespace dabnn {
 // The quantiser: per block, A = the largest finite |x|, scale = 2^e with e = max(-126, least integer with A <= 448 * 2^e),
 // q = e4m3(x * 2^-e).  A power of two, so that the product is exact, the rounding to e4m3 the only one, and a block's values
 // the same whichever order or width they are computed in; 8-bit floats lose nothing by it but the lowest binade.
-// One pass over the data: a thread keeps its values in registers between the maximum and the conversion.  Bound by HBM.
+// One pass over the data: a thread keeps its values in registers between the maximum and the conversion.  Bound by HBM: 8192 x
+// 4096 bf16 by rows 17.7 us (5.8 TB/s), fp32 by blocks of 128 x 128 27.4 us (6.1 TB/s).
 
 // the scale's bits from those of A (fp32), 448 = 1.75 * 2^8; the reciprocal's bits are (254 << 23) - scale
 __device__ __forceinline__ uint32_t f8_scale_bits(uint32_t top) {
