@@ -60,6 +60,7 @@ struct HaloParams {
                                   // (streamed weights only: a CTA then copies its rows out of every box image)
     int resident, pair;
     int narrow;                   // see EpiOut
+    int constants_first;          // weights, a and b are older than every launch that may still be running: they are read ahead of the wait for it
 };
 
 template <bool PAIR, bool POOL>
@@ -107,6 +108,7 @@ __global__ void __launch_bounds__(HL_THREADS, 1)
     }
     if (p.imgs == 2 && tid < p.hslots * 4)   // the zero pixel behind the second image's halo (never written again)
         sts128(smem_u32(halo0) + (tid >> 2) * p.halo_stride + (p.img_pitch + (p.rows + 2) * p.P) * 64 + (tid & 3) * 16, 0u, 0u, 0u, 0u);
+    if (!p.constants_first) grid_dependency_wait();
     if (tid < TC5_MAX_N) {
         pop[tid] = epi_pop(tid < n_this ? __ldg(reinterpret_cast<const int*>(p.w_img + u8_weight_image_bytes(p.N, nboxes)) + n0 + tid) : 0);
         const bool have = p.a && tid < n_this;
@@ -121,7 +123,7 @@ __global__ void __launch_bounds__(HL_THREADS, 1)
     // this CTA's rows of its channel block's box images
     const unsigned char* wsrc = p.w_img + (size_t)(n0 / TC5_MAX_N) * nboxes * gbox_bytes + (size_t)(n0 % TC5_MAX_N) * 64;
     grid_launch_dependents();
-    if (warp != 1) grid_dependency_wait();   // the weight loader reads constants only and may run ahead of the previous kernel's end
+    if (warp != 1) grid_dependency_wait();   // the weight loader reads constants only: where those are old it may run ahead of the previous kernel's end
 
     if (warp == 0) {
         // =========================== halo loads: one lane ===========================

@@ -220,7 +220,7 @@ bool bconv_u8_pool_supported(int n, int h, int w, int cin, int cout, int kh, int
 int bconv_u8_block_impl(const unsigned char* in_u8, const unsigned char* w_img, const float* a, const float* b,
                         const float* shortcut, float* out_f32, unsigned char* out_u8, uint64_t* out_bits, int n, int h, int w,
                         int cin, int cout, int kh, int kw, int pad_h, int pad_w, int stride_h, int stride_w,
-                        cudaStream_t stream, float* pool_out) {
+                        cudaStream_t stream, float* pool_out, bool constants_first) {
     DABNN_REQUIRE(in_u8 && w_img, DABNN_ERR_ARG, "bconv_u8: null pointer");
     DABNN_REQUIRE((a == nullptr) == (b == nullptr), DABNN_ERR_ARG, "bconv_u8: a and b go together");
     DABNN_REQUIRE(out_f32 || out_u8 || out_bits, DABNN_ERR_ARG, "bconv_u8: no output requested");
@@ -254,7 +254,7 @@ int bconv_u8_block_impl(const unsigned char* in_u8, const unsigned char* w_img, 
         q.B = n; q.OH = hp.OH; q.OW = hp.OW; q.N = cout; q.cw = cin / 64; q.P = hp.P; q.imgs = hp.imgs; q.img_pitch = hp.img_pitch; q.nb = hp.nb;
         q.rows = hp.rows; q.tiles_per_img = hp.tiles_per_img; q.ntiles = hp.ntiles;
         q.hslots = hp.hslots; q.halo_stride = hp.halo_stride; q.wstages = hp.wstages; q.wb = hp.wb;
-        q.resident = hp.resident; q.pair = hp.pair; q.narrow = narrow;
+        q.resident = hp.resident; q.pair = hp.pair; q.narrow = narrow; q.constants_first = constants_first;
         const int tiles_n = (cout + hp.nb - 1) / hp.nb;
         const int per_n = std::max(1, sm_count() / tiles_n);
         const int nunits = hp.pair ? (hp.ntiles + 1) / 2 : hp.ntiles;
@@ -271,7 +271,7 @@ int bconv_u8_block_impl(const unsigned char* in_u8, const unsigned char* w_img, 
     p.B = n; p.OH = pl.OH; p.OW = pl.OW; p.N = cout;
     p.kh = kh; p.kw = kw; p.pad_h = pad_h; p.pad_w = pad_w; p.stride = stride_h; p.cw = cin / 64;
     p.rows = pl.rows; p.imgs = pl.imgs; p.tiles_per_img = pl.tiles_per_img; p.ntiles = pl.ntiles;
-    p.G = pl.G; p.stages = pl.stages; p.wb = pl.wb; p.nboxes = pl.nboxes; p.resident = pl.resident; p.wide = pl.wide; p.pair = pl.pair; p.nbc = pl.nbc; p.narrow = narrow;
+    p.G = pl.G; p.stages = pl.stages; p.wb = pl.wb; p.nboxes = pl.nboxes; p.resident = pl.resident; p.wide = pl.wide; p.pair = pl.pair; p.nbc = pl.nbc; p.narrow = narrow; p.constants_first = constants_first;
     const int tiles_n = (cout + pl.nbc - 1) / pl.nbc;
     const int per_n = std::max(1, sm_count() / tiles_n);
     const int nunits = pl.pair ? (pl.ntiles + 1) / 2 : pl.ntiles;

@@ -60,6 +60,7 @@ struct U8Params {
     int wide;                     // cin % 128 == 0: one TMA load covers two K boxes (128-byte rows, SWIZZLE_128B)
     int pair;                     // two pixel tiles share every weight stage (streamed weights: halves their bytes)
     int narrow;                   // see EpiOut
+    int constants_first;          // weights, a and b are older than every launch that may still be running: they are read ahead of the wait for it
     int nbc;                      // output channels per CTA: TC5_MAX_N, or 64 / 32 when there are too few tiles to fill the SMs
                                   // (streamed weights only: a CTA then copies its rows out of every box image)
 };
@@ -171,6 +172,7 @@ __global__ void __launch_bounds__(U8_THREADS, 1)
         asm volatile("fence.mbarrier_init.release.cluster;" ::);
         s_abort = 0;
     }
+    if (!p.constants_first) grid_dependency_wait();
     if (tid < TC5_MAX_N) {
         pop[tid] = epi_pop(tid < n_this ? __ldg(reinterpret_cast<const int*>(p.w_img + u8_weight_image_bytes(p.N, p.nboxes)) + n0 + tid) : 0);
         const bool have = p.a && tid < n_this;

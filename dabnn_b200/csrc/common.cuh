@@ -40,6 +40,8 @@ int sm_count();
 // kernel before it in the stream is still draining, runs its set-up (shared memory, tensor memory, barriers, constant
 // weights) and then calls grid_dependency_wait(), which returns once everything launched before it has completed and is
 // visible.  Only kernels that make that call before they touch activations may be launched this way.
+// A launch cannot know what its caller's earlier launches write: only a Net, whose weights were complete before its run began,
+// lets a kernel read them ahead of the wait (constants_first).
 extern int g_overlap_launches;   // 1 (default): on; dabnn_debug_set_launch_overlap
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 // Lets the kernel that follows in the stream (if it was launched with launch_overlapped) start as soon as every CTA of

@@ -198,6 +198,7 @@ __global__ void __launch_bounds__(FS_THREADS, 1)
         const uint32_t pa = smem_u32(patch);
         for (int i = tid; i < g.slots * g.slot_bytes / 16; i += FS_THREADS) sts128f(pa + i * 16, 0.f, 0.f, 0.f, 0.f);
     }
+    if (!p.constants_first) grid_dependency_wait();
     if (tid < FS_N) {
         const bool in = tid < n_this;
         chan_bias[tid] = (in && p.bias) ? __ldg(p.bias + n0 + tid) : 0.f;

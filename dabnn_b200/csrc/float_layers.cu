@@ -368,6 +368,7 @@ struct FconvParams {
     float* out;
     int relu, n, h, w, cin, cout, kh, kw, pad_h, pad_w, stride_h, stride_w, dil_h, dil_w, oh, ow;
     const float* wgt_rem;   // or null: w - trunc_tf32(w) for every weight, computed once by fconv_split_weights (fconv_gemm.cuh)
+    int constants_first;    // weights, bias, a and b are older than every launch that may still be running: they are read ahead of the wait for it
 };
 
 __global__ void __launch_bounds__(FNT, 2) fconv_kernel(const FconvParams p) {
@@ -658,7 +659,7 @@ bool fconv_pool_supported(int n, int h, int w, int cin, int cout, int kh, int kw
 
 int fconv_pool_impl(const float* in, const float* weight, const float* bias, const float* a, const float* b, int relu, float* pool_out,
                     unsigned char* pool_u8, int n, int h, int w, int cin, int cout, int kh, int kw, int pad_h, int pad_w, int stride_h,
-                    int stride_w, cudaStream_t stream) {
+                    int stride_w, cudaStream_t stream, bool constants_first) {
     DABNN_REQUIRE(in && weight && pool_out, DABNN_ERR_ARG, "fconv_pool: null pointer");
     DABNN_REQUIRE((a == nullptr) == (b == nullptr), DABNN_ERR_ARG, "fconv_pool: a and b go together");
     DABNN_REQUIRE(fconv_pool_supported(n, h, w, cin, cout, kh, kw, pad_h, pad_w, stride_h, stride_w), DABNN_ERR_SHAPE,
@@ -666,7 +667,7 @@ int fconv_pool_impl(const float* in, const float* weight, const float* bias, con
     DABNN_REQUIRE(((reinterpret_cast<uintptr_t>(pool_out) | reinterpret_cast<uintptr_t>(pool_u8)) & 15) == 0 && (reinterpret_cast<uintptr_t>(in) & 3) == 0,
                   DABNN_ERR_ARG, "fconv_pool: outputs must be 16-byte aligned");
     const int oh = conv_out_dim(h, pad_h, 1, kh, stride_h), ow = conv_out_dim(w, pad_w, 1, kw, stride_w);
-    const FconvParams prm{in, weight, bias, a, b, pool_out, relu, n, h, w, cin, cout, kh, kw, pad_h, pad_w, stride_h, stride_w, 1, 1, oh, ow};
+    const FconvParams prm{in, weight, bias, a, b, pool_out, relu, n, h, w, cin, cout, kh, kw, pad_h, pad_w, stride_h, stride_w, 1, 1, oh, ow, nullptr, constants_first};
     FsGeom geom;
     DABNN_REQUIRE(fconv_stem_plan(prm, geom, true), DABNN_ERR_SHAPE, "fconv_pool: shape not taken by the fused convolution + pooling kernel");
     const int ny = (cout + FS_N - 1) / FS_N;
@@ -729,7 +730,7 @@ bool fconv_uses_weight_remainders(int cin, int cout, int kh, int kw, int pad_h, 
 
 int fconv_impl(const float* in, const float* weight, const float* bias, const float* a, const float* b, int relu,
                float* out, int n, int h, int w, int cin, int cout, int kh, int kw, int pad_h, int pad_w,
-               int stride_h, int stride_w, int dil_h, int dil_w, cudaStream_t stream, const float* weight_rem) {
+               int stride_h, int stride_w, int dil_h, int dil_w, cudaStream_t stream, const float* weight_rem, bool constants_first) {
     DABNN_REQUIRE(in && weight && out, DABNN_ERR_ARG, "fconv: null pointer");
     DABNN_REQUIRE(n > 0 && h > 0 && w > 0 && cin > 0 && cout > 0 && kh > 0 && kw > 0 && stride_h > 0 &&
                       stride_w > 0 && dil_h > 0 && dil_w > 0 && pad_h >= 0 && pad_w >= 0, DABNN_ERR_ARG,
@@ -741,7 +742,7 @@ int fconv_impl(const float* in, const float* weight, const float* bias, const fl
     DABNN_REQUIRE((reinterpret_cast<uintptr_t>(out) & 7) == 0, DABNN_ERR_ARG, "fconv: output must be 8-byte aligned");
     dim3 grid((n * oh * ow + FTM - 1) / FTM, (cout + FTN - 1) / FTN);
     const FconvParams prm{in, weight, bias, a, b, out, relu, n, h, w, cin, cout, kh, kw, pad_h, pad_w,
-                          stride_h, stride_w, dil_h, dil_w, oh, ow, (reinterpret_cast<uintptr_t>(weight_rem) & 15) == 0 ? weight_rem : nullptr};
+                          stride_h, stride_w, dil_h, dil_w, oh, ow, (reinterpret_cast<uintptr_t>(weight_rem) & 15) == 0 ? weight_rem : nullptr, constants_first};
     auto al16 = [](const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0; };
     const bool pointwise = fconv_is_pointwise(kh, kw, pad_h, pad_w, stride_h, stride_w);
     if (fconv_gemm_takes(cin, cout, kh, kw, pad_h, pad_w, stride_h, stride_w, dil_h, dil_w) && al16(in) && al16(weight) && al16(out) && al16(bias) &&

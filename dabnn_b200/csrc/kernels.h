@@ -52,10 +52,13 @@ int binarize_u8_impl(const float* in, unsigned char* out, size_t count, cudaStre
 // pool_out (optional): the 2x2 stride-2 average pooling of the fp32 result, fp32 [n][oh / 2][ow / 2][cout], written by the
 // same kernel; bconv_u8_pool_supported tells for which shapes (3x3, stride 1, padding 1, even height and width).
 bool bconv_u8_pool_supported(int n, int h, int w, int cin, int cout, int kh, int kw, int pad_h, int pad_w, int stride_h, int stride_w);
+// constants_first (here and for the float convolutions below): what w_img, a and b point to was complete before the launch before
+// this one began - a model's weights are - and may be read while that launch still runs.  Calls from outside may hand over what
+// the launch before them computes, so they wait first (0.5 - 0.7 us of a chain of calls, the thin-input convolution's 1.3).
 int bconv_u8_block_impl(const unsigned char* in_u8, const unsigned char* w_img, const float* a, const float* b,
                         const float* shortcut, float* out_f32, unsigned char* out_u8, uint64_t* out_bits, int n, int h, int w,
                         int cin, int cout, int kh, int kw, int pad_h, int pad_w, int stride_h, int stride_w,
-                        cudaStream_t stream, float* pool_out = nullptr);
+                        cudaStream_t stream, float* pool_out = nullptr, bool constants_first = false);
 int bconv_u8_status(int* status);
 
 // Device addresses (on the current device) of the words in which the tensor-core kernels record the code of a
@@ -75,7 +78,8 @@ int elementwise_chain(const float* x, const float* a, const float* b, const floa
 int fconv_tc5_status(int* status);
 int fconv_impl(const float* in, const float* weight, const float* bias, const float* a, const float* b,
                int relu, float* out, int n, int h, int w, int cin, int cout, int kh, int kw, int pad_h,
-               int pad_w, int stride_h, int stride_w, int dil_h, int dil_w, cudaStream_t stream, const float* weight_rem = nullptr);
+               int pad_w, int stride_h, int stride_w, int dil_h, int dil_w, cudaStream_t stream, const float* weight_rem = nullptr,
+               bool constants_first = false);
 // weight_rem (optional, 16-byte aligned): the remainders w - trunc_tf32(w) of constant weights, computed once by
 // fconv_split_weights; the GEMM kernel (fconv_gemm.cuh) then loads them by TMA instead of recomputing them for every tile.
 // fconv_uses_weight_remainders tells for which convolutions they are read.
@@ -87,7 +91,7 @@ bool fconv_uses_weight_remainders(int cin, int cout, int kh, int kw, int pad_h, 
 bool fconv_pool_supported(int n, int h, int w, int cin, int cout, int kh, int kw, int pad_h, int pad_w, int stride_h, int stride_w);
 int fconv_pool_impl(const float* in, const float* weight, const float* bias, const float* a, const float* b, int relu, float* pool_out,
                     unsigned char* pool_u8, int n, int h, int w, int cin, int cout, int kh, int kw, int pad_h, int pad_w, int stride_h,
-                    int stride_w, cudaStream_t stream);
+                    int stride_w, cudaStream_t stream, bool constants_first = false);
 
 // Max pooling that also emits the signs of its output (the first binary conv's input), packed and / or as bytes.
 int maxpool_impl(const float* in, float* out, uint64_t* out_bits, int n, int h, int w, int c, int kh, int kw,

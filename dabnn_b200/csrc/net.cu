@@ -954,7 +954,7 @@ int NetImpl::run_plan(int batch) {
                                              o.in2 >= 0 ? f32(o.in2) : nullptr, f32(o.out),
                                              o.write_bits && ob.u8 ? bytes(o.out) : nullptr,
                                              o.write_bits && !ob.u8 ? bits(o.out) : nullptr, batch, ib.h, ib.w, ib.c, ob.c, o.kh,
-                                             o.kw, o.pad_h, o.pad_w, o.stride_h, o.stride_w, stream, o.out2 >= 0 ? f32(o.out2) : nullptr);
+                                             o.kw, o.pad_h, o.pad_w, o.stride_h, o.stride_w, stream, o.out2 >= 0 ? f32(o.out2) : nullptr, true);
                     break;
                 }
                 rc = bconv_block_impl(bits(o.in), static_cast<const uint64_t*>(o.w->dev), o.w->count,
@@ -978,7 +978,7 @@ int NetImpl::run_plan(int batch) {
                                 o.bias ? static_cast<const float*>(o.bias->dev) : nullptr,
                                 o.a ? static_cast<const float*>(o.a->dev) : nullptr,
                                 o.b ? static_cast<const float*>(o.b->dev) : nullptr, o.relu, f32(o.out), batch, ib.h,
-                                ib.w, ib.c, ob.c, o.kh, o.kw, o.pad_h, o.pad_w, o.stride_h, o.stride_w, 1, 1, stream, o.w_rem);
+                                ib.w, ib.c, ob.c, o.kh, o.kw, o.pad_h, o.pad_w, o.stride_h, o.stride_w, 1, 1, stream, o.w_rem, true);
                 break;
             }
             case OpKind::FConvPool: {
@@ -988,7 +988,7 @@ int NetImpl::run_plan(int batch) {
                                      o.a ? static_cast<const float*>(o.a->dev) : nullptr,
                                      o.b ? static_cast<const float*>(o.b->dev) : nullptr, o.relu, f32(o.out),
                                      o.write_bits && ob.u8 ? bytes(o.out) : nullptr, batch, ib.h, ib.w, ib.c, ob.c, o.kh, o.kw,
-                                     o.pad_h, o.pad_w, o.stride_h, o.stride_w, stream);
+                                     o.pad_h, o.pad_w, o.stride_h, o.stride_w, stream, true);
                 break;
             }
             case OpKind::Chain:

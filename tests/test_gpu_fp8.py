@@ -401,3 +401,48 @@ def test_classifier_head(ops, m, classes, k):
     sw = np.repeat(np.repeat(R.quantize(values(w), 128)[1], 128, 0)[:classes], 128, 1)[:, :k] * 2.0 ** -10
     ex, ew = np.maximum(ax * 2.0 ** -4, sx), np.maximum(aw * 2.0 ** -4, sw)
     R.close(values(logits), exact, tol + ex @ aw.T + ax @ ew.T + ex @ ew.T)
+
+
+# ---------------------------------------------------------------------------------------------- results as another launch's constants
+def test_results_as_parameters_of_the_next_launch(ops):
+    """Factors, offsets, biases and weights that the launch just before computes (a product of few rows, which leaves most SMs
+    free; a pooling): the same bits as with a synchronisation between the two."""
+    g = torch.Generator().manual_seed(41)
+    cout, k = 128, 16384
+    x8 = ops.binarize_u8(torch.randn((2, 14, 14, 128), generator=g).cuda())
+    bits = ops.pack_mat(torch.randn((cout, 3, 3, 128), generator=g).cuda())
+    we = ops.bconv_u8_expand_weights(bits, cout, 18)
+    image, stem = torch.randn((1, 224, 224, 3), generator=g).cuda(), torch.randn((64, 7, 7, 3), generator=g).cuda()
+    assert ops.fconv_maxpool_supported(1, 224, 224, 3, 64, 7, 7, 3, 3, 2, 2)
+    w = [ops.fp8_quantize_weights((torch.randn((n, k), generator=g) * k ** -0.5).cuda()) for n in (cout, 64, 64 * 7 * 7 * 3)]
+    features = [ops.fp8_quantize(torch.randn((2, k), generator=g).cuda()) for _ in range(4)]
+    thin = [ops.fp8_quantize(torch.randn((2, k), generator=g).cuda()) for _ in range(4)]
+    maps = [torch.randn((1, 8, 8, cout), generator=g).cuda() for _ in range(4)]
+
+    def chain(wait):
+        out = []
+
+        def sync(t):
+            if wait:
+                torch.cuda.synchronize()
+            return t
+
+        for i in range(12):
+            f = features[i % 4]
+            c = sync(ops.fp8_gemm(*f, *w[0]))
+            out.append(ops.bconv_u8_block(x8, we, cout, 3, 3, 1, 1, 1, 1, c[0], c[1])[0])
+            c = sync(ops.fp8_gemm(*f, *w[0]))
+            out.append(ops.bconv_u8_block(x8, we, cout, 3, 3, 1, 1, 2, 2, c[1], c[0])[0])
+            c = sync(ops.avepool(maps[i % 4], 8, 8, 0, 0, 8, 8)).view(cout)
+            out.append(ops.bconv_u8_block(x8, we, cout, 3, 3, 1, 1, 1, 1, c, c)[0])
+            c = sync(ops.fp8_gemm(*f, *w[1]))
+            out.append(ops.fconv_maxpool(image, stem, c[1], 3, 3, 2, 2, c[0], c[1])[0])
+            c = sync(ops.fp8_gemm(*f, *w[1]))
+            out.append(ops.fconv(image, stem, c[0], 3, 3, 2, 2))
+            c = sync(ops.fp8_gemm(*thin[i % 4], *w[2]))
+            out.append(ops.fconv(image, c[0].view(64, 7, 7, 3), None, 3, 3, 2, 2))
+            sync(None)
+        return out
+
+    for got, expected in zip(chain(False), chain(True)):
+        assert torch.equal(got, expected)
