@@ -249,6 +249,8 @@ static int f8_launch(const Fp8Params& p, int splits, const CUtensorMap& lane_map
     return DABNN_OK;
 }
 
+static int g_give_up_group = -1, g_give_up_rank = 0;   // dabnn_debug_fp8_give_up
+
 template <typename T>
 static int f8_gemm(Fp8Params p, const uint8_t* a, long long lda, const uint8_t* b, long long ldb, int k, cudaStream_t stream) {
     const int nt = f8_columns(p.M, p.N), rows_m = nt <= 64 ? nt : nt == 128 ? 128 : 256, rows_n = nt <= 64 ? 128 : nt;
@@ -257,6 +259,8 @@ static int f8_gemm(Fp8Params p, const uint8_t* a, long long lda, const uint8_t* 
     DABNN_REQUIRE(ntiles < (1ll << 30), DABNN_ERR_SHAPE, "fp8_gemm: too many outputs");
     p.ntiles = (int)ntiles;
     p.nkb = (k + F8_BLOCK - 1) / F8_BLOCK;
+    p.give_up_group = g_give_up_group;
+    p.give_up_rank = g_give_up_rank;
     CUtensorMap w_map{}, x_map{};
     if (k > 0) {   // a single row's pitch is of no account, but the descriptor wants one
         const unsigned long long whole = ((unsigned long long)k + 15) / 16 * 16;
@@ -345,4 +349,11 @@ extern "C" int dabnn_fp8_gemm(const uint8_t* a, long long lda, const float* a_sc
     if (c_type == DABNN_F32) return f8_gemm<float>(p, a, lda, b, ldb, k, stream);
     if (c_type == DABNN_F16) return f8_gemm<__half>(p, a, lda, b, ldb, k, stream);
     return f8_gemm<__nv_bfloat16>(p, a, lda, b, ldb, k, stream);
+}
+
+extern "C" int dabnn_debug_fp8_give_up(int group, int rank) {
+    DABNN_REQUIRE(group >= -1 && rank >= 0 && rank < F8_MAX_SPLIT, DABNN_ERR_ARG, "fp8_give_up: group must be -1 or more, rank 0 - 7");
+    g_give_up_group = group;
+    g_give_up_rank = rank;
+    return DABNN_OK;
 }

@@ -21,7 +21,9 @@
 // 14 us); at few rows HBM and set-up (1 x 16384 x 16384 54 us, 5.0 TB/s; 1 x 8192 x 4096 9.4 us, 3.6 TB/s).
 //
 // Every wait on an mbarrier is bounded; one that gives up records a code (51 loader, 52 / 53 MMA warp waiting for an
-// accumulator / a stage, 54 epilogue, 55 factors), raises the CTA's abort flag, and the CTA frees its tensor memory and returns.
+// accumulator / a stage, 54 epilogue, 55 factors) and raises the abort flag, in both CTAs of a pair, at which every role stops.
+// What was started goes on without them: before the tensor memory is freed and a CTA leaves, the instructions issued so far and
+// the loads still on their way, the other CTA's among them, are waited for, again with a limit.
 #pragma once
 #include "bcontract_tc5.cuh"
 #include "scalar_types.cuh"
@@ -43,6 +45,7 @@ struct Fp8Params {
     int M, N, nkb;                                     // activation rows, weight rows, blocks of K
     int tiles_n, ntiles;                               // tiles along the weight rows; all tiles
     int tma_out;                                       // rows of c begin on 16-byte boundaries: tensor stores
+    int give_up_group, give_up_rank;                   // dabnn_debug_fp8_give_up: which group of factors of which CTA of a team is held to have run out of time; none: -1
 };
 
 template <int NT>
@@ -60,14 +63,14 @@ struct Fp8Cfg {                                        // NT: columns of a tile
     static constexpr int SMEM = 1024 + STAGES * STAGE_BYTES + OUT_BYTES;
 };
 
-// A bounded wait of a whole warp
+// A bounded wait of a whole warp (that no abort flag ends where it is null)
 __device__ __forceinline__ bool f8_wait(uint32_t bar, uint32_t parity, const volatile int* abort_flag) {
     for (uint32_t it = 0; it < TC5_SPIN_LIMIT; it++) {
         uint32_t done;
         asm volatile("{\n\t.reg .pred P1;\n\tmbarrier.try_wait.parity.shared::cta.b64 P1, [%1], %2;\n\tselp.b32 %0, 1, 0, P1;\n\t}"
                      : "=r"(done) : "r"(bar), "r"(parity) : "memory");
         if (__all_sync(0xffffffffu, done)) return true;
-        if ((it & 255u) == 255u && __any_sync(0xffffffffu, *abort_flag)) return false;
+        if (abort_flag && (it & 255u) == 255u && __any_sync(0xffffffffu, *abort_flag)) return false;
     }
     return false;
 }
@@ -133,6 +136,27 @@ __device__ __forceinline__ void f8_cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// Waits for the loads that nothing else waits for after an abort; called by one thread, of a pair's first CTA.  Load n of a CTA
+// belongs to phase n / STAGES of its stage's barrier - for a pair the first CTA's, which announces the bytes of both.  The
+// loaders stop by themselves: of the loads that only one of the two has issued, the first CTA's are announced with bytes of the
+// other that will not come, which are counted as having come, and the other's have not been announced at all, which is made up
+// for.  (At most STAGES loads lie between the two: both wait for the same instructions to free a stage.)
+template <bool PAIR, int STAGES, int BYTES>
+__device__ __forceinline__ void f8_await_loads(uint64_t* bar_full, const int* loads) {
+    const int mine = *loads;
+    int other = mine;
+    if (PAIR) asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(other) : "r"(f8_in_cta(smem_u32(loads), 1)) : "memory");
+    const int all = max(mine, other), never = 0;
+#pragma unroll 1
+    for (int n = min(mine, other); n < all; n++) {
+        const uint32_t bar = smem_u32(&bar_full[n % STAGES]);
+        if (n < mine) asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(BYTES) : "memory");
+        else asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(BYTES) : "memory");
+    }
+#pragma unroll 1
+    for (int n = max(0, all - STAGES); n < all; n++) mbar_wait(&bar_full[n % STAGES], (n / STAGES) & 1, &never);
+}
+
 // SPLIT: the CTAs of a cluster share one tile (the grid then has one cluster per tile); otherwise a CTA walks the tiles
 template <int NT, bool SPLIT, typename T>
 __global__ void __launch_bounds__(Fp8Cfg<NT>::THREADS, Fp8Cfg<NT>::CTAS_PER_SM)
@@ -141,7 +165,7 @@ __global__ void __launch_bounds__(Fp8Cfg<NT>::THREADS, Fp8Cfg<NT>::CTAS_PER_SM)
     using Cfg = Fp8Cfg<NT>;
     extern __shared__ unsigned char smem_dyn[];
     __shared__ __align__(8) uint64_t bar_full[Cfg::STAGES], bar_empty[Cfg::STAGES], bar_acc_full[2], bar_acc_empty[2];
-    __shared__ __align__(8) uint64_t bar_factor_full[F8_GROUPS], bar_factor_empty[F8_GROUPS];
+    __shared__ __align__(8) uint64_t bar_factor_full[F8_GROUPS], bar_factor_empty[F8_GROUPS], bar_issued;
     __shared__ __align__(16) float factors[F8_GROUPS][F8_GROUP][Cfg::FACTORS];
     __shared__ uint32_t tmem_base_s;
     __shared__ int s_abort, s_loads;
@@ -169,6 +193,7 @@ __global__ void __launch_bounds__(Fp8Cfg<NT>::THREADS, Fp8Cfg<NT>::CTAS_PER_SM)
         for (int i = 0; i < Cfg::STAGES; i++) { mbar_init(&bar_full[i], 1); mbar_init(&bar_empty[i], 1); }
         for (int i = 0; i < F8_GROUPS; i++) { mbar_init(&bar_factor_full[i], 1); mbar_init(&bar_factor_empty[i], Cfg::EPI_WARPS); }
         for (int i = 0; i < 2; i++) { mbar_init(&bar_acc_full[i], 1); mbar_init(&bar_acc_empty[i], (PAIR ? 2 : 1) * Cfg::EPI_WARPS); }
+        mbar_init(&bar_issued, 1);                     // every instruction of the MMA warp is complete
         asm volatile("fence.mbarrier_init.release.cluster;" ::);
         s_abort = 0;
         s_loads = 0;
@@ -181,6 +206,11 @@ __global__ void __launch_bounds__(Fp8Cfg<NT>::THREADS, Fp8Cfg<NT>::CTAS_PER_SM)
     // In this order: a kernel that this lets start may read its constants at once, and they may come from a launch before this one.
     grid_dependency_wait();
     grid_launch_dependents();
+    auto give_up = [&](int code) {                     // a wait ran out: nothing of the team's tile can be finished
+        atomicCAS(&g_fp8_status, 0, code);
+        s_abort = 1;
+        if (PAIR) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(f8_in_cta(smem_u32(&s_abort), rank ^ 1)), "r"(1) : "memory");
+    };
     if (warp < Cfg::EPI_WARP0) {
         // a pair's 20 warps have 96 registers each at launch: these four give 32 of theirs to the epilogue's sixteen, whose sums and two
         // chunks of an accumulator take 96
@@ -194,8 +224,7 @@ __global__ void __launch_bounds__(Fp8Cfg<NT>::THREADS, Fp8Cfg<NT>::CTAS_PER_SM)
                     const int tm = tile / p.tiles_n, tn = tile - tm * p.tiles_n;
                     for (int kb = kb0; kb < kb1; kb++) {
                         if (use >= 1 && !mbar_wait(&bar_empty[s], (use - 1) & 1, abort_flag)) {
-                            atomicCAS(&g_fp8_status, 0, 51);
-                            s_abort = 1;
+                            give_up(51);
                             ok = false;
                             break;
                         }
@@ -222,14 +251,12 @@ __global__ void __launch_bounds__(Fp8Cfg<NT>::THREADS, Fp8Cfg<NT>::CTAS_PER_SM)
                 for (int kb = kb0; kb < kb1; kb++, i++) {
                     const int acc = i & 1;
                     if (i >= 2 && !f8_wait(smem_u32(&bar_acc_empty[acc]), ((i >> 1) - 1) & 1, abort_flag)) {
-                        atomicCAS(&g_fp8_status, 0, 52);
-                        s_abort = 1;
+                        give_up(52);
                         ok = false;
                         break;
                     }
                     if (!f8_wait(smem_u32(&bar_full[s]), par, abort_flag)) {
-                        atomicCAS(&g_fp8_status, 0, 53);
-                        s_abort = 1;
+                        give_up(53);
                         ok = false;
                         break;
                     }
@@ -244,6 +271,7 @@ __global__ void __launch_bounds__(Fp8Cfg<NT>::THREADS, Fp8Cfg<NT>::CTAS_PER_SM)
                     __syncwarp();
                     if (++s == Cfg::STAGES) { s = 0; par ^= 1u; }
                 }
+            if (leader && (!PAIR || rank == 0)) f8_commit<PAIR>(smem_u32(&bar_issued));
         } else if (warp == 2) {
             // =========================== factors as * bs ===========================
             // FEW: a lane has the columns lane, lane + 32; else rows lane + 32 j of the tile, each with the bs of every 128 columns
@@ -267,9 +295,9 @@ __global__ void __launch_bounds__(Fp8Cfg<NT>::THREADS, Fp8Cfg<NT>::CTAS_PER_SM)
                         b += p.bs_block;
                     }
                     const int slot = i % F8_GROUPS;
-                    if (i >= F8_GROUPS && !f8_wait(smem_u32(&bar_factor_empty[slot]), (i / F8_GROUPS - 1) & 1, abort_flag)) {
-                        atomicCAS(&g_fp8_status, 0, 55);
-                        s_abort = 1;
+                    if ((i >= F8_GROUPS && !f8_wait(smem_u32(&bar_factor_empty[slot]), (i / F8_GROUPS - 1) & 1, abort_flag)) ||
+                        (i == p.give_up_group && rank == p.give_up_rank)) {
+                        give_up(55);
                         ok = false;
                         break;
                     }
@@ -314,8 +342,7 @@ __global__ void __launch_bounds__(Fp8Cfg<NT>::THREADS, Fp8Cfg<NT>::CTAS_PER_SM)
                     in_group = 0;
                 }
                 if (!there || !f8_wait(acc_full + acc * 8, acc_par, abort_flag)) {
-                    atomicCAS(&g_fp8_status, 0, 54);
-                    s_abort = 1;
+                    give_up(54);
                     ok = false;
                     break;
                 }
@@ -470,12 +497,14 @@ __global__ void __launch_bounds__(Fp8Cfg<NT>::THREADS, Fp8Cfg<NT>::CTAS_PER_SM)
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    if (s_abort && (!PAIR || rank == 0) && threadIdx.x == 0) {   // loads may be on their way still (a pair's all arrive at the first CTA's barriers)
-        const int never = 0;
-        for (int i = max(0, s_loads - Cfg::STAGES); i < s_loads; i++) mbar_wait(&bar_full[i % Cfg::STAGES], (i / Cfg::STAGES) & 1, &never);
-    }
+    if (warp == 1) f8_wait(smem_u32(&bar_issued), 0, nullptr);   // the instructions read and write both CTAs' memory, and arrive at their barriers
     __syncwarp();
-    if (PAIR) f8_cluster_sync();                       // no CTA leaves while the other arrives at its barriers
+    if (PAIR) f8_cluster_sync();                       // neither arrives at the other's barriers any more, nor raises its flag: the two are the same
+    if (s_abort) {
+        if (threadIdx.x == 0 && (!PAIR || rank == 0)) f8_await_loads<PAIR, Cfg::STAGES, Cfg::STAGE_BYTES>(bar_full, &s_loads);
+        __syncwarp();
+        if (PAIR) f8_cluster_sync();                   // neither leaves while loads for it are on their way
+    }
     if (warp == 1) {
         __syncwarp();
         if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS));

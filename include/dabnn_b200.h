@@ -372,6 +372,11 @@ int dabnn_debug_set_launch_overlap(int on);
  * without stalling a GPU. */
 int dabnn_debug_raise_engine_status(int which, int code);
 
+/* Test hook: from the next call on, a product of 8-bit floats whose tile's team (a CTA, a pair, a cluster) has a CTA `rank` that
+ * comes to its group `group` of four blocks of k holds that CTA's wait for the factors to have given up there: it records 55 and
+ * winds down as after a real one, its result is unusable.  group -1: off (the default). */
+int dabnn_debug_fp8_give_up(int group, int rank);
+
 #ifdef __cplusplus
 }
 #endif

@@ -446,3 +446,31 @@ def test_results_as_parameters_of_the_next_launch(ops):
 
     for got, expected in zip(chain(False), chain(True)):
         assert torch.equal(got, expected)
+
+
+@pytest.mark.parametrize("m,n,k,places", [
+    (1, 300, 300, [(0, 0)]), (1, 8192, 4096, [(0, 0), (1, 3)]), (20, 700, 2048, [(0, 1)]), (50, 600, 4096, [(0, 0), (0, 7)]), (50, 600, 1280, [(2, 0)]),
+    (200, 4100, 2048, [(0, 0), (2, 0)]), (1000, 2600, 4096, [(0, 0), (0, 1), (1, 1), (4, 0), (7, 1)]), (2300, 4200, 1100, [(1, 0), (3, 1), (4, 0), (5, 1)])])
+def test_winding_down_after_a_wait_that_gave_up(ops, m, n, k, places):
+    """Every kind of tile, either CTA of a pair, early and late: the call ends, its code is there to be read, and what follows
+    it in the stream, at once, is as it always is.  (A wait is declared to have run out; nothing is made to stall.)"""
+    from dabnn_b200 import capi
+    lib = capi.load()
+    a, sa, b, sb, bias = operands(m, n, k, 17)
+    args = (R.f8(a), dev(sa), R.f8(b), dev(sb), dev(bias))
+    expected = ops.fp8_gemm(*args)
+    assert ops.engine_status() == 0
+    try:
+        for group, rank in places:
+            for _ in range(3):
+                capi.check(lib.dabnn_debug_fp8_give_up(group, rank))
+                ops.fp8_gemm(*args)
+                capi.check(lib.dabnn_debug_fp8_give_up(-1, 0))
+                after = ops.fp8_gemm(*args)
+                torch.cuda.synchronize()
+                assert ops.engine_status() == 55, (group, rank)
+                capi.check(lib.dabnn_debug_raise_engine_status(3, 0))
+                assert torch.equal(after, expected), (group, rank)
+    finally:
+        capi.check(lib.dabnn_debug_fp8_give_up(-1, 0))
+    assert lib.dabnn_debug_fp8_give_up(-2, 0) == 1 and lib.dabnn_debug_fp8_give_up(0, 8) == 1 and lib.dabnn_debug_fp8_give_up(0, -1) == 1
