@@ -84,6 +84,7 @@ _SIGNATURES = {
     "dabnn_measure_engine_peak": [_i, C.POINTER(C.c_double)],
     "dabnn_measure_tf32_peak": [C.POINTER(C.c_double)],
     "dabnn_engine_status": [C.POINTER(_i)],
+    "dabnn_collect_engine_status": [C.POINTER(_i)],
     "dabnn_last_engine": [],
     "dabnn_debug_raise_engine_status": [_i, _i],
     "dabnn_debug_fp8_give_up": [_i, _i],

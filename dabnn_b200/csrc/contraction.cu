@@ -340,10 +340,14 @@ int dabnn::contraction_status_word(int** addr) {
 
 extern "C" int dabnn_last_engine(void) { return g_last_engine; }
 
+static int status_word(int which, int** word) {
+    return which == 0 ? contraction_status_word(word) : which == 1 ? fconv_status_word(word) : which == 2 ? bconv_u8_status_word(word) : fp8_status_word(word);
+}
+
 extern "C" int dabnn_debug_raise_engine_status(int which, int code) {
     DABNN_REQUIRE(which >= 0 && which <= 3, DABNN_ERR_ARG, "raise_engine_status: which must be 0, 1, 2 or 3");
     int* word = nullptr;
-    const int rc = which == 0 ? contraction_status_word(&word) : which == 1 ? fconv_status_word(&word) : which == 2 ? bconv_u8_status_word(&word) : fp8_status_word(&word);
+    const int rc = status_word(which, &word);
     if (rc) return rc;
     DABNN_CUDA_OK(cudaMemcpy(word, &code, sizeof(int), cudaMemcpyHostToDevice));
     return DABNN_OK;
@@ -367,5 +371,23 @@ extern "C" int dabnn_engine_status(int* status) {
         if (rc) return rc;
         DABNN_CUDA_OK(cudaMemcpy(status, word, sizeof(int), cudaMemcpyDeviceToHost));
     }
+    return DABNN_OK;
+}
+
+extern "C" int dabnn_collect_engine_status(int* status) {
+    DABNN_REQUIRE(status, DABNN_ERR_ARG, "null output");
+    DABNN_CUDA_OK(cudaDeviceSynchronize());
+    int first = 0;
+    for (int which = 0; which < 4; which++) {   // in the order in which dabnn_engine_status reads them
+        int *word = nullptr, code = 0;
+        const int rc = status_word(which, &word);
+        if (rc) return rc;
+        DABNN_CUDA_OK(cudaMemcpy(&code, word, sizeof(int), cudaMemcpyDeviceToHost));
+        if (!code) continue;
+        DABNN_CUDA_OK(cudaMemset(word, 0, sizeof(int)));
+        if (!first) first = code;
+    }
+    if (first) DABNN_CUDA_OK(cudaDeviceSynchronize());   // the words are clear before the next launch may raise one
+    *status = first;
     return DABNN_OK;
 }

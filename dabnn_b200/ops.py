@@ -437,10 +437,12 @@ def measure_tf32_peak():
     return v.value
 
 
-def engine_status():
-    """0, or the code of the first bounded wait that gave up inside a tcgen05 kernel (synchronises)."""
+def engine_status(collect=False):
+    """0, or the code of the first bounded wait that gave up inside a tcgen05 kernel (synchronises).  collect: the codes are
+    cleared as well, so that the next answer tells of later calls (see dabnn_collect_engine_status)."""
     v = C.c_int()
-    check(capi.load().dabnn_engine_status(C.byref(v)))
+    lib = capi.load()
+    check((lib.dabnn_collect_engine_status if collect else lib.dabnn_engine_status)(C.byref(v)))
     return v.value
 
 

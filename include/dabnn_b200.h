@@ -349,9 +349,14 @@ int dabnn_measure_tf32_peak(double* flops_per_second);
  * 3 / 4 MMA thread (accumulator never released / stage never filled); float convolution 11 producers, 12 epilogue, 13 / 14 MMA thread (accumulator /
  * stage), 15 / 16 row loader and its consumers; byte-activation engine 21 loader, 22 / 23 MMA thread
  * (accumulator / stage or resident weights), 24 epilogue; 8-bit float product 51 loader, 52 / 53 MMA warp (accumulator /
- * stage), 54 epilogue, 55 factors.  A Net collects (and clears) the words itself at the
- * end of every run and reports them as DABNN_ERR_TIMEOUT from dabnn_net_wait / _sync / _get_blob. */
+ * stage), 54 epilogue, 55 factors.  A Net collects (and clears) the words of the first three itself at the end of every run and
+ * reports them as DABNN_ERR_TIMEOUT from dabnn_net_wait / _sync / _get_blob; the product's (51 - 55) no Net collects.  A code
+ * stays until it is collected: by a Net, or by dabnn_collect_engine_status. */
 int dabnn_engine_status(int* status);
+
+/* dabnn_engine_status that also clears what it has read, the words of all four: whoever launches kernels through the
+ * entry points above learns by it whether a wait gave up since the last time it was called. */
+int dabnn_collect_engine_status(int* status);
 
 /* Which engine (DABNN_ENGINE_POPC ... DABNN_ENGINE_TCGEN05) the calling thread's most recent dabnn_bgemm /
  * dabnn_bconv / dabnn_bconv_block / dabnn_binconv_forward call actually launched: DABNN_ENGINE_TCGEN05 requests

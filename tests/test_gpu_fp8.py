@@ -474,3 +474,35 @@ def test_winding_down_after_a_wait_that_gave_up(ops, m, n, k, places):
     finally:
         capi.check(lib.dabnn_debug_fp8_give_up(-1, 0))
     assert lib.dabnn_debug_fp8_give_up(-2, 0) == 1 and lib.dabnn_debug_fp8_give_up(0, 8) == 1 and lib.dabnn_debug_fp8_give_up(0, -1) == 1
+
+
+def test_collecting_the_code_of_a_wait_that_gave_up(ops):
+    """Codes planted from the host: reading leaves them, collecting clears the words of every kernel, a Net's run only its own."""
+    from dabnn_b200 import capi
+    lib = capi.load()
+    for which, code in ((0, 3), (1, 12), (2, 21), (3, 53)):
+        capi.check(lib.dabnn_debug_raise_engine_status(which, code))
+        assert ops.engine_status() == code and ops.engine_status() == code
+        assert ops.engine_status(collect=True) == code
+        assert ops.engine_status(collect=True) == 0 and ops.engine_status() == 0
+    for which, code in ((0, 3), (3, 51)):
+        capi.check(lib.dabnn_debug_raise_engine_status(which, code))
+    assert ops.engine_status(collect=True) == 3 and ops.engine_status() == 0        # one answer for all that happened before it
+    capi.check(lib.dabnn_debug_raise_engine_status(3, 52))
+    from dabnn_b200.bireal import OUTPUT_BLOB, build_bireal18
+    from dabnn_b200.dab_format import write_dab
+    from dabnn_b200.net import Net
+    net = Net.create()
+    net.max_batch = 1
+    net.read_buf(write_dab(build_bireal18(image_hw=32, num_classes=10)))
+    net.run(torch.randn((1, 32, 32, 3), device="cuda")).get_blob(OUTPUT_BLOB)
+    net.close()
+    assert ops.engine_status(collect=True) == 52 and ops.engine_status() == 0
+    # a code that a kernel itself has raised
+    a, sa, b, sb, bias = operands(3, 300, 300, 18)
+    capi.check(lib.dabnn_debug_fp8_give_up(0, 0))
+    try:
+        ops.fp8_gemm(R.f8(a), dev(sa), R.f8(b), dev(sb))
+    finally:
+        capi.check(lib.dabnn_debug_fp8_give_up(-1, 0))
+    assert ops.engine_status(collect=True) == 55 and ops.engine_status() == 0

@@ -135,3 +135,8 @@ def test_python_refusals_by_device_and_kind(pretend):
                    pretend(torch.zeros((4, 1), dtype=torch.int64)), pretend(torch.zeros(8, dtype=torch.int64))[::2], pretend(torch.zeros(4, dtype=torch.int64), 1)):
         with pytest.raises(TypeError):
             ops.logprobs(x, labels)
+
+
+def test_collect_engine_status_refusals(lib):
+    assert lib.dabnn_collect_engine_status(None) == ARG
+    assert lib.dabnn_debug_fp8_give_up(-2, 0) == ARG and lib.dabnn_debug_fp8_give_up(0, 8) == ARG and lib.dabnn_debug_fp8_give_up(0, -1) == ARG
