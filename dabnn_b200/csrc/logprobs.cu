@@ -32,6 +32,7 @@ constexpr int LP_WARPS = 8, LP_MAX_CLUSTER = 8;        // warps of a CTA that sh
 constexpr int LP_ROWS = 4;                             // warps of a CTA that have a row each
 constexpr float LP_LOG2E = 1.4426950408889634f, LP_LN2 = 0.6931471805599453f;
 constexpr float LP_FLOOR = -1e30f;                     // a difference below it has e^d = 0; keeps d e^d a number
+constexpr float LP_GONE = 1024.f;                      // a maximum this far below another (in units of ln 2) has e^d = 0; its product with a sum of as many terms as a row has is a number
 
 // fp32 -> unsigned, order preserved; a NaN is the largest, the zeros are one value, nothing is 0
 __device__ __forceinline__ uint32_t order_key(float x) {
@@ -86,7 +87,7 @@ __device__ __forceinline__ float2 two_fma(float2 a, float2 b, float2 c) {
 struct Part {
     float m, s, w;
     __device__ __forceinline__ void raise(float to) {   // to >= m
-        const float delta = m == -INFINITY ? 0.f : fminf((to - m) * LP_LOG2E, -LP_FLOOR), scale = exp2_fast(-delta);
+        const float delta = m == -INFINITY ? 0.f : fminf((to - m) * LP_LOG2E, LP_GONE), scale = exp2_fast(-delta);
         w = scale * (w - delta * s);
         s *= scale;
         m = to;

@@ -246,3 +246,25 @@ def test_net_logprobs(ops):
         with pytest.raises(ValueError):
             net.logprobs(OUTPUT_BLOB, labels=[1, 2, 3])
         net.close()
+
+
+def test_rows_of_hundreds_of_millions_of_classes(ops):
+    """One class far above 4 10^8 equal ones, in the part of the row that is joined last: each part of the row before it holds
+    a sum of e^0 of 5 10^7, whose product with the distance between the maxima is beyond fp32."""
+    classes, top = 400_000_000, 7 * 1024 + 5
+    x = torch.full((1, classes), -1e30, dtype=torch.bfloat16, device="cuda")
+    x[0, top] = 1e30
+    low, high = float(x[0, 0]), float(x[0, top])
+    lp, rank, ent, tlp, ti = ops.logprobs(x, torch.tensor([top], device="cuda"), 2)
+    assert lp.item() == 0 and rank.item() == 0 and ent.item() == 0
+    assert ti.tolist() == [[top, 0]] and tlp[0, 0].item() == 0
+    R.close(tlp[0, 1:].cpu(), [low - high], 2.0 ** -23 * (high - low))
+    x[0, top] = -1e30                                                  # all alike
+    lp, rank, ent, tlp, ti = ops.logprobs(x, torch.tensor([top], device="cuda"), 2)
+    # 4e8 terms of 1: sums of whole numbers below 2^24 in a lane, 64 lanes' worth of roundings above; a logarithm
+    expected = np.log(float(classes))
+    tol = 72 * 2.0 ** -24 + expected * 2.0 ** -22
+    R.close(lp.cpu(), [-expected], tol)
+    R.close(ent.cpu(), [expected], tol)
+    assert rank.item() == top and ti.tolist() == [[0, 1]]
+    R.close(tlp.cpu(), [[-expected, -expected]], tol)
