@@ -1185,6 +1185,8 @@ extern "C" int dabnn_net_logprobs(dabnn_net* net, const char* name, const int64_
     DABNN_REQUIRE(n.cur_batch > 0, DABNN_ERR_STATE, "logprobs: the net has not been run");
     DABNN_REQUIRE((long long)dims[0] * dims[1] * dims[2] <= INT_MAX, DABNN_ERR_SHAPE, "logprobs: too many rows");
     DABNN_REQUIRE(top >= 0 && top <= DABNN_LOGPROBS_MAX_TOP && top <= dims[3], DABNN_ERR_ARG, "logprobs: top must be between 0 and the smaller of 64 and the classes");
+    DABNN_REQUIRE(labels || (!label_logprob && !label_rank), DABNN_ERR_ARG, "logprobs: a label's outputs without labels");
+    DABNN_REQUIRE(top == 0 || (top_logprob && top_index), DABNN_ERR_ARG, "logprobs: null pointer");
     const size_t rows = (size_t)dims[0] * dims[1] * dims[2], tops = rows * top;
     // 8-byte values first: labels, rank, top index | label log probability, entropy, top log probability
     const size_t rank_at = rows * 8, index_at = rank_at + rows * 8, lp_at = index_at + tops * 8, entropy_at = lp_at + rows * 4,

@@ -311,7 +311,7 @@ int dabnn_net_wait(dabnn_net* net, int ticket);
 int dabnn_net_get_blob_bits(dabnn_net* net, const char* name, int dims[4], const uint64_t** device_ptr,
                             uint64_t* to_host, size_t host_words);
 /* dabnn_logprobs on a blob of the last run (fp32 logits; the rows are its pixels, batch * h * w of them, c the classes) with
- * host arrays: labels [rows] or NULL, outputs as there, each may be NULL.  Waits for the run and for the results.  Which
+ * host arrays: labels [rows] or NULL; outputs as there, refused and left out as there.  Waits for the run and for the results.  Which
  * blobs can be scored: those dabnn_net_get_blob returns.  The first call allocates a device buffer that later ones of at
  * most its size use again. */
 int dabnn_net_logprobs(dabnn_net* net, const char* name, const int64_t* labels, float* label_logprob, int64_t* label_rank,

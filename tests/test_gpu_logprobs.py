@@ -268,3 +268,38 @@ def test_rows_of_hundreds_of_millions_of_classes(ops):
     R.close(ent.cpu(), [expected], tol)
     assert rank.item() == top and ti.tolist() == [[0, 1]]
     R.close(tlp.cpu(), [[-expected, -expected]], tol)
+
+
+def test_net_logprobs_refuses_what_logprobs_refuses(ops):
+    """A label's outputs without labels, alternatives without a place for them: refused, nothing is written; what may be left out
+    is left out."""
+    import ctypes as C
+    from dabnn_b200 import capi
+    from dabnn_b200.bireal import OUTPUT_BLOB, build_bireal18
+    from dabnn_b200.dab_format import write_dab
+    from dabnn_b200.net import Net
+    lib = capi.load()
+    net = Net.create()
+    net.max_batch = 3
+    net.read_buf(write_dab(build_bireal18(image_hw=32, num_classes=10)))
+    net.run(torch.randn((3, 32, 32, 3), device="cuda"))
+    logits = torch.from_numpy(net.get_blob(OUTPUT_BLOB).reshape(3, 10)).cuda()
+    labels = np.array([1, 9, 4], np.int64)
+    lab_dev = torch.from_numpy(labels).cuda()
+    want = [t.cpu().numpy() for t in ops.logprobs(logits, torch.from_numpy(labels).cuda(), 2)]
+    for given in range(64):
+        lab, top = bool(given & 1), 2 if given & 2 else 0
+        out = [np.full(3, -77.0, np.float32), np.full(3, -77, np.int64), np.full(3, -77.0, np.float32), np.full((3, 2), -77.0, np.float32), np.full((3, 2), -77, np.int64)]
+        have = [bool(given & 4), bool(given & 8), True, bool(given & 16), bool(given & 32)]
+        ptr = [o.ctypes.data_as(C.c_void_p) if h else None for o, h in zip(out, have)]
+        rc = lib.dabnn_net_logprobs(net._h, OUTPUT_BLOB.encode(), labels.ctypes.data_as(C.c_void_p) if lab else None, *ptr, top)
+        keep = [torch.from_numpy(o).cuda() for o in out]
+        dev = [t.data_ptr() if h else None for t, h in zip(keep, have)]
+        assert rc == lib.dabnn_logprobs(logits.data_ptr(), 0, 10, lab_dev.data_ptr() if lab else None, 3, 10, *dev, top, ops._stream())
+        torch.cuda.synchronize()
+        refused = (not lab and (have[0] or have[1])) or (top and not (have[3] and have[4]))
+        assert (rc == 1) if refused else (rc == 0), given
+        for i, o in enumerate(out):
+            written = not refused and have[i] and (i < 3 or top)
+            np.testing.assert_array_equal(o, want[i] if written else np.full_like(o, -77))
+    net.close()
