@@ -62,6 +62,7 @@ _SIGNATURES = {
     "dabnn_fp8_quantize": [_p, _i, _l, _p, _l, _p, _l, _l, _i, _i, _i, _p],
     "dabnn_fp8_gemm": [_p, _l, _p, _l, _l, _p, _l, _p, _l, _l, _p, _p, _i, _l, _i, _i, _i, _p],
     "dabnn_logprobs": [_p, _i, _l, _p, _i, _i, _p, _p, _p, _p, _p, _i, _p],
+    "dabnn_logprobs_grouped": [_p, _i, _l, _l, _p, _l, _i, _i, _i, _p, _p, _p, _p, _p, _i, _p],
     "dabnn_net_create": [C.POINTER(_p)],
     "dabnn_net_destroy": [_p],
     "dabnn_net_set_flags": [_p, _i, _i, _i],

@@ -165,11 +165,22 @@ struct Best {
 
 struct LogprobsParams {
     const void* logits;
-    long long ld;
+    long long ld, ld_group;                            // between rows of a group, between groups
     const int64_t* labels;
+    long long label_group;
     float *label_logprob, *entropy, *top_logprob;
     int64_t *label_rank, *top_index;
-    int rows, classes, top;
+    int group_rows, rows, classes, top;
+    // where the logits and the label of a warp's row lie (the address from one lane: known to be the same in all, it stays in
+    // uniform registers; 4096 rows of 65536 bf16 132 us otherwise)
+    template <typename T>
+    __device__ __forceinline__ const T* place(int row, int64_t& label) const {
+        const int g = row < group_rows ? 0 : row / group_rows, i = row - g * group_rows;
+        label = labels ? labels[g * label_group + i] : -1;
+        const unsigned long long at = reinterpret_cast<unsigned long long>(static_cast<const T*>(logits) + g * ld_group + i * ld);
+        const uint32_t lo = __shfl_sync(0xffffffffu, (uint32_t)at, 0), hi = __shfl_sync(0xffffffffu, (uint32_t)(at >> 32), 0);
+        return reinterpret_cast<const T*>((unsigned long long)hi << 32 | lo);
+    }
 };
 
 __device__ __forceinline__ void lp_write(const LogprobsParams& p, long long row, int64_t label, float mine, const Part& all, unsigned long long before) {
@@ -485,12 +496,13 @@ __global__ void __launch_bounds__(LP_ROWS * 32, 7) logprobs_warp_kernel(const Lo
     const long long row = (long long)blockIdx.x * LP_ROWS + warp;
     grid_dependency_wait();
     if (row >= p.rows) return;
-    const int64_t label = p.labels ? p.labels[row] : -1;
+    int64_t label;
+    const T* const logits = p.place<T>((int)row, label);
     float mine;
     Part all;
     unsigned before;
     Best<ENTRIES> best;
-    lp_scan<T, ENTRIES, false>(p, static_cast<const T*>(p.logits) + row * p.ld, label, mine, 0, 1, &stash[ENTRIES ? warp : 0], nullptr, all, before, best);
+    lp_scan<T, ENTRIES, false>(p, logits, label, mine, 0, 1, &stash[ENTRIES ? warp : 0], nullptr, all, before, best);
     if (lane == 0) lp_write(p, row, label, mine, all, before);
     if (ENTRIES)
 #pragma unroll
@@ -512,13 +524,13 @@ __global__ void __launch_bounds__(LP_WARPS * 32, 4) logprobs_team_kernel(const L
     if (threadIdx.x < LP_WARPS) shared.reach[threadIdx.x] = 0;
     __syncthreads();
     grid_dependency_wait();
-    const int64_t label = p.labels ? p.labels[row] : -1;
+    int64_t label;
+    const T* const logits = p.place<T>((int)row, label);
     float mine;
     Part all;
     unsigned before;
     Best<ENTRIES> best;
-    lp_scan<T, ENTRIES, true>(p, static_cast<const T*>(p.logits) + row * p.ld, label, mine, warp * ctas + rank, LP_WARPS * ctas, &stash[ENTRIES ? warp : 0], &shared, all,
-                              before, best);
+    lp_scan<T, ENTRIES, true>(p, logits, label, mine, warp * ctas + rank, LP_WARPS * ctas, &stash[ENTRIES ? warp : 0], &shared, all, before, best);
     if (lane == 0) { parts[warp] = all; before_s[warp] = before; }
     if (ENTRIES)
 #pragma unroll
@@ -646,18 +658,24 @@ using namespace dabnn;
 
 extern "C" int dabnn_logprobs(const void* logits, int type, long long ld, const int64_t* labels, int rows, int classes, float* label_logprob,
                               int64_t* label_rank, float* entropy, float* top_logprob, int64_t* top_index, int top, dabnn_stream_t s) {
+    return dabnn_logprobs_grouped(logits, type, ld, 0, labels, 0, rows > 0 ? rows : 1, rows, classes, label_logprob, label_rank, entropy, top_logprob, top_index, top, s);
+}
+
+extern "C" int dabnn_logprobs_grouped(const void* logits, int type, long long ld, long long ld_group, const int64_t* labels, long long label_group, int group_rows,
+                                      int rows, int classes, float* label_logprob, int64_t* label_rank, float* entropy, float* top_logprob, int64_t* top_index,
+                                      int top, dabnn_stream_t s) {
     DABNN_REQUIRE(type >= DABNN_F32 && type <= DABNN_BF16, DABNN_ERR_ARG, "logprobs: unknown type");
-    DABNN_REQUIRE(rows >= 0 && classes >= 1, DABNN_ERR_ARG, "logprobs: bad dims");
+    DABNN_REQUIRE(rows >= 0 && classes >= 1 && group_rows >= 1, DABNN_ERR_ARG, "logprobs: bad dims");
     DABNN_REQUIRE(classes < INT_MAX / 2, DABNN_ERR_SHAPE, "logprobs: too many classes");
     DABNN_REQUIRE(top >= 0 && top <= DABNN_LOGPROBS_MAX_TOP && top <= classes, DABNN_ERR_ARG, "logprobs: top must be between 0 and the smaller of 64 and the classes");
     if (rows == 0) return DABNN_OK;
     DABNN_REQUIRE(labels || (!label_logprob && !label_rank), DABNN_ERR_ARG, "logprobs: a label's outputs without labels");
     DABNN_REQUIRE(top == 0 || (top_logprob && top_index), DABNN_ERR_ARG, "logprobs: null pointer");
     DABNN_REQUIRE(logits, DABNN_ERR_ARG, "logprobs: null pointer");
-    DABNN_REQUIRE(ld >= classes || rows == 1, DABNN_ERR_SHAPE, "logprobs: the row pitch is below the classes");
+    DABNN_REQUIRE(ld >= classes || rows == 1 || group_rows == 1, DABNN_ERR_SHAPE, "logprobs: the row pitch is below the classes");
     DABNN_REQUIRE((reinterpret_cast<uintptr_t>(logits) & (type == DABNN_F32 ? 3 : 1)) == 0, DABNN_ERR_ARG, "logprobs: misaligned pointer");
     const cudaStream_t stream = static_cast<cudaStream_t>(s);
-    const LogprobsParams p{logits, ld, labels, label_logprob, entropy, top_logprob, label_rank, top_index, rows, classes, top};
+    const LogprobsParams p{logits, ld, ld_group, labels, label_group, label_logprob, entropy, top_logprob, label_rank, top_index, group_rows, rows, classes, top};
     auto launch = [&](auto tag) {
         using T = decltype(tag);
         return top == 0 ? lp_launch<T, 0>(p, stream) : top <= 32 ? lp_launch<T, 1>(p, stream) : lp_launch<T, 2>(p, stream);

@@ -318,8 +318,22 @@ def _here(*tensors):
             raise TypeError("expected CUDA tensors on the current device")
 
 
+def _levels(shape, strides):
+    """Dimensions, outermost first, as (size, stride) levels: those that walk memory in equal steps are one."""
+    levels = []
+    for size, stride in zip(shape, strides):
+        if size == 1:
+            continue
+        if levels and levels[-1][1] == size * stride:
+            levels[-1] = (levels[-1][0] * size, stride)
+        else:
+            levels.append((size, stride))
+    return levels
+
+
 def _rows(t, what):
-    """(rows, columns, pitch) of a tensor taken as rows along its last dimension: a matrix with any row pitch, or contiguous."""
+    """(rows, columns, pitch) of a tensor taken as rows along its last dimension, which lie at equal steps: a matrix with any row
+    pitch, a contiguous tensor, one whose rows alone have a pitch."""
     if t.dim() == 2:
         rows, cols = t.shape
         if cols <= 1 or t.stride(1) == 1:
@@ -331,7 +345,14 @@ def _rows(t, what):
         if rows >= 1 << 31 or cols >= 1 << 31:
             raise ValueError(f"{what}: too large a matrix")
         return rows, cols, cols
-    raise TypeError(f"{what}: expected a matrix with unit stride along its rows, or a contiguous tensor")
+    elif t.dim() > 2 and (t.shape[-1] <= 1 or t.stride(-1) == 1):
+        levels = _levels(t.shape[:-1], t.stride()[:-1])
+        if len(levels) < 2:
+            rows, cols = t.shape[:-1].numel(), t.shape[-1]
+            if rows >= 1 << 31 or cols >= 1 << 31:
+                raise ValueError(f"{what}: too large a matrix")
+            return rows, cols, levels[0][1] if levels else cols
+    raise TypeError(f"{what}: expected rows of unit stride that lie at equal steps")
 
 
 def _fp8_quantize(x, block_rows):
@@ -396,30 +417,71 @@ def fp8_gemm(a, a_scales, b, b_scales, bias=None, out_dtype=torch.float32):
     return c if lead is None else c.unflatten(0, lead) if lead else c[0]
 
 
+def _grouped_rows(logits, labels):
+    """(rows, classes, pitch of rows, rows of a group, pitch of groups, pitch of the groups' labels) of logits whose rows, or
+    whose labels, do not all lie at equal steps."""
+    lead, classes = logits.shape[:-1], logits.shape[-1]
+    rows = lead.numel()
+    if rows >= 1 << 31 or classes >= 1 << 31:
+        raise ValueError("logprobs: too large a matrix")
+    levels = _levels(lead, logits.stride()[:-1])
+    if (classes > 1 and logits.stride(-1) != 1) or len(levels) > 2:
+        raise TypeError("logprobs: expected rows of unit stride, in groups that lie at equal steps")
+    # rows: groups of `size`, `ld` apart; labels: groups of `label_size`
+    size, ld = levels[-1] if levels else (rows, classes)
+    ld_group = levels[0][1] if len(levels) == 2 else 0
+    label_size, label_group = rows, 0
+    if labels is not None and not labels.is_contiguous():
+        levels = _levels(labels.shape, labels.stride())
+        if len(levels) == 1 and labels.dim() > 1 and labels.shape[-1] == 1:
+            levels.append((1, 1))
+        if len(levels) != 2 or levels[1][1] != 1:
+            raise TypeError("logprobs: expected labels that lie side by side, or in groups that do")
+        label_size, label_group = levels[1][0], levels[0][1]
+    if size == rows:
+        size, ld_group = label_size, label_size * ld
+    elif label_size == rows:
+        label_group = size
+    elif size != label_size:
+        raise TypeError("logprobs: the groups of rows and of labels differ")
+    return rows, classes, ld, size, ld_group, label_group
+
+
 def logprobs(logits, labels=None, top=0):
     """Scores rows of logits [..., classes] (fp32, fp16, bf16) -> (label_logprob, label_rank, entropy, top_logprob, top_index):
     ln softmax of the class in `labels` (int64 [...]) and how many classes come before it, the entropy, and the `top`
     likeliest classes with their ln softmax [..., top]; None for what was not asked.  Equal logits rank by index; a
-    negative label is ignored (0 and -1).  Rows with -inf, NaN and other labels: see dabnn_logprobs."""
+    negative label is ignored (0 and -1).  Rows with -inf, NaN and other labels: see dabnn_logprobs.
+    Rows may have a pitch, and so may groups of rows of one size, labels included (see dabnn_logprobs_grouped):
+    logprobs(logits[:, :-1], tokens[:, 1:]) scores a batch of sequences where they lie."""
     _here(logits, labels)
     kind = _FLOATS.get(logits.dtype)
     if kind is None:
         raise TypeError("logprobs: expected fp32, fp16 or bf16")
-    rows, classes, ld = _rows(logits, "logprobs")
     lead = logits.shape[:-1]
-    lp = rank = tlp = ti = None
+    lp = rank = tlp = ti = groups = None
+    if (logits.dim() == 2 or logits.is_contiguous()) and (labels is None or labels.is_contiguous()):
+        rows, classes, ld = _rows(logits, "logprobs")
+    else:
+        rows, classes, ld, *groups = _grouped_rows(logits, labels)
     if labels is not None:
-        if labels.dtype != torch.int64 or labels.shape != lead or not labels.is_contiguous():
-            raise TypeError("logprobs: expected contiguous int64 labels, one for each row")
-        rank, lp = torch.empty_like(labels), torch.empty_like(labels, dtype=torch.float32)
+        if labels.dtype != torch.int64 or labels.shape != lead:
+            raise TypeError("logprobs: expected int64 labels, one for each row")
+        rank = torch.empty_like(labels, memory_format=torch.contiguous_format)
+        lp = torch.empty_like(rank, dtype=torch.float32)
         entropy = torch.empty_like(lp)
     else:
         entropy = logits.new_empty(lead, dtype=torch.float32)
     if top:
         tlp = torch.empty(*lead, max(top, 0), dtype=torch.float32, device=logits.device)
         ti = torch.empty_like(tlp, dtype=torch.int64)
-    check(capi.load().dabnn_logprobs(logits.data_ptr(), kind, ld, _ptr(labels), rows, classes, _ptr(lp), _ptr(rank), entropy.data_ptr(), _ptr(tlp),
-                                     _ptr(ti), top, _stream()))
+    if groups:
+        group_rows, ld_group, label_group = groups
+        check(capi.load().dabnn_logprobs_grouped(logits.data_ptr(), kind, ld, ld_group, _ptr(labels), label_group, group_rows, rows, classes, _ptr(lp),
+                                                 _ptr(rank), entropy.data_ptr(), _ptr(tlp), _ptr(ti), top, _stream()))
+    else:
+        check(capi.load().dabnn_logprobs(logits.data_ptr(), kind, ld, _ptr(labels), rows, classes, _ptr(lp), _ptr(rank), entropy.data_ptr(), _ptr(tlp),
+                                         _ptr(ti), top, _stream()))
     return lp, rank, entropy, tlp, ti
 
 

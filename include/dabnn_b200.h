@@ -258,6 +258,15 @@ int dabnn_logprobs(const void* logits, int type, long long ld, const int64_t* la
                    float* label_logprob, int64_t* label_rank, float* entropy, float* top_logprob, int64_t* top_index,
                    int top, dabnn_stream_t s);
 
+/* dabnn_logprobs of rows that lie in groups of group_rows: row g * group_rows + i is at logits + g * ld_group + i * ld, its
+ * label at labels[g * label_group + i]; the outputs are dense.  All positions but the last of each of `batch` sequences,
+ * scored against the tokens that follow: ld = classes, ld_group = len * classes, labels + 1, label_group = len, group_rows =
+ * len - 1, rows = batch * (len - 1).  Groups may overlap or be one another. */
+int dabnn_logprobs_grouped(const void* logits, int type, long long ld, long long ld_group, const int64_t* labels,
+                           long long label_group, int group_rows, int rows, int classes, float* label_logprob,
+                           int64_t* label_rank, float* entropy, float* top_logprob, int64_t* top_index, int top,
+                           dabnn_stream_t s);
+
 /* ---------------------------------------------------------------------------------------------
  * Net level: reference dabnn/net.h:22-66 class bnn::Net.
  * ------------------------------------------------------------------------------------------- */

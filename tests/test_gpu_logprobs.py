@@ -303,3 +303,58 @@ def test_net_logprobs_refuses_what_logprobs_refuses(ops):
             written = not refused and have[i] and (i < 3 or top)
             np.testing.assert_array_equal(o, want[i] if written else np.full_like(o, -77))
     net.close()
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("batch,length,classes,top", [(3, 5, 1000, 5), (2, 3, 40001, 20), (700, 3, 301, 3), (40, 60, 4100, 0), (1, 7, 50, 2), (5, 2, 9001, 64)])
+def test_sequences_where_they_lie(ops, batch, length, classes, top, kind):
+    """All positions but the last, of a vocabulary with padding, against the tokens that follow; what is not a row is NaN."""
+    g = torch.Generator().manual_seed(batch * length + classes)
+    store = torch.full((batch, length, classes + 3), NAN, dtype=TYPES[kind], device="cuda")
+    tokens = torch.randint(0, classes, (batch, length), generator=g).cuda()
+    x, labels = store[:, :-1, 1:classes + 1], tokens[:, 1:]
+    x.copy_((torch.randn((batch, length - 1, classes), generator=g) * 3).cuda())
+    tokens[:, 0] = 1 << 40
+    (lp, rank, ent, tlp, ti), (tol, etol, ttol) = R.logprobs(x.float().cpu().numpy().reshape(-1, classes), labels.cpu().numpy().reshape(-1), top)
+    lead = (batch, length - 1)
+    for logits in (x, x.contiguous()):
+        for lab in (labels, labels.contiguous()):
+            got = ops.logprobs(logits, lab, top)
+            assert got[0].shape == got[1].shape == got[2].shape == lead
+            np.testing.assert_array_equal(got[1].cpu(), rank.reshape(lead))
+            R.close(got[0].cpu(), lp.reshape(lead), tol.reshape(lead))
+            R.close(got[2].cpu(), ent.reshape(lead), etol.reshape(lead))
+            if top:
+                np.testing.assert_array_equal(got[4].cpu(), ti.reshape(*lead, top))
+                R.close(got[3].cpu(), tlp.reshape(*lead, top), ttol.reshape(*lead, top))
+    R.close(ops.logprobs(x)[2].cpu(), ent.reshape(lead), etol.reshape(lead))
+
+
+def test_groups_beyond_32_bits_and_groups_that_are_one(ops):
+    """Groups that begin beyond 2^32 elements of the base; one sequence's logits for every sequence's tokens; refused shapes."""
+    classes, pitch = 1000, 1 << 31
+    store = torch.zeros(2 * pitch + 4 * classes, dtype=torch.bfloat16, device="cuda")
+    x = store.as_strided((3, 2, classes), (pitch, classes + 8, 1))
+    flat = rows_of(6, classes, 13, "bf16")[0]
+    x.copy_(flat.view(3, 2, classes))
+    tokens = torch.arange(12, device="cuda").view(3, 4) * 80
+    got, want = ops.logprobs(x, tokens[:, 1:3], 5), R.logprobs(flat.float().cpu().numpy(), tokens[:, 1:3].reshape(-1).cpu().numpy(), 5)
+    np.testing.assert_array_equal(got[1].cpu().reshape(-1), want[0][1])
+    R.close(got[0].cpu().reshape(-1), want[0][0], want[1][0])
+    np.testing.assert_array_equal(got[4].cpu().reshape(6, 5), want[0][4])
+    one = flat[:4].view(1, 4, classes).expand(3, 4, classes)[:, :-1]
+    got = ops.logprobs(one, tokens[:, 1:])
+    for b in range(3):
+        (lp, rank, _, _, _), (tol, _, _) = R.logprobs(flat[:3].float().cpu().numpy(), tokens[b, 1:].cpu().numpy(), 0)
+        np.testing.assert_array_equal(got[1][b].cpu(), rank)
+        R.close(got[0][b].cpu(), lp, tol)
+    with pytest.raises(TypeError):
+        ops.logprobs(x.transpose(1, 2))
+
+
+def test_quantise_rows_with_a_pitch(ops):
+    """Leading dimensions whose rows alone have a pitch: the same bytes as of a copy."""
+    x = torch.randn((3, 5, 400), device="cuda")
+    for part in (x[..., :300], x[..., 3:260], x[:, 2:3, 8:]):
+        for a, b in zip(ops.fp8_quantize(part), ops.fp8_quantize(part.contiguous())):
+            assert a.shape == b.shape and torch.equal(a.float(), b.float())

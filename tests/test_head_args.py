@@ -140,3 +140,96 @@ def test_python_refusals_by_device_and_kind(pretend):
 def test_collect_engine_status_refusals(lib):
     assert lib.dabnn_collect_engine_status(None) == ARG
     assert lib.dabnn_debug_fp8_give_up(-2, 0) == ARG and lib.dabnn_debug_fp8_give_up(0, 8) == ARG and lib.dabnn_debug_fp8_give_up(0, -1) == ARG
+
+
+# logits [..., classes] and labels [...] as a program slices them; None: refused
+B = torch.zeros((4, 9, 30))
+L = torch.zeros((4, 9), dtype=torch.int64)
+SLICES = {
+    "all but the last position": (B[:, :-1], L[:, 1:]),
+    "the middle, a padded vocabulary": (B[:, 2:7, :25], L[:, 1:6]),
+    "padded vocabulary": (B[..., :25], L),
+    "padded vocabulary, labels of all but the first": (B[:, :8, 3:25].contiguous(), L[:, 1:]),
+    "labels made whole": (B[:, :-1], L[:, 1:].contiguous()),
+    "logits made whole": (B[:, :-1].contiguous(), L[:, 1:]),
+    "no labels": (B[1:, 3:], None),
+    "one position of each": (B[:, 4], L[:, 4].contiguous()),
+    "one position of each, kept": (B[:, 4:5], L[:, 4:5].contiguous()),
+    "two positions": (B[:, 3:4], L[:, 5:6]),
+    "two positions, the same logits": (B[:1, 3:4].expand(4, 1, 30), L[:, 5:6]),
+    "every other sequence": (B[::2, :-1], L[::2, 1:]),
+    "one sequence": (B[1:2, :-1], L[2:3, 1:]),
+    "one sequence, flat": (B[1, :-1], L[2, 1:]),
+    "the same logits for each": (B[:1].expand(4, 9, 30)[:, 1:], L[:, 1:]),
+    "four levels that are two": (torch.zeros((2, 3, 5, 7, 10))[:, 1:], torch.zeros((2, 2, 5, 7), dtype=torch.int64)),
+    "one row": (B[2, 3, 4:], L[1, 2]),
+    "none": (B[:0, :-1], L[:0, 1:]),
+    "a gap in two dimensions": (torch.zeros((2, 3, 4, 5, 6))[:, :2, :3, :4], None),
+    "classes apart": (B.transpose(1, 2)[:, :-1], None),
+    "labels apart": (B[:, :-1], L.t().contiguous().t()[:, 1:]),
+    "labels apart, flat": (B[:, 4], L[:, 4]),
+    "groups of other sizes": (torch.zeros((3, 4, 5, 30))[:, :, 1:], torch.zeros((3, 5, 5), dtype=torch.int64)[:, 1:].view(3, 4, 5)),
+}
+REFUSED = {"a gap in two dimensions", "classes apart", "labels apart", "labels apart, flat", "groups of other sizes"}
+
+
+@pytest.mark.parametrize("name", SLICES)
+def test_where_rows_and_labels_are_read(name, monkeypatch):
+    """The addresses a call hands over are those of its tensors' rows, in their order."""
+    calls = []
+
+    class Recorder:
+        def __getattr__(self, function):
+            return lambda *args: calls.append((function, args)) or 0
+
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda device: 0, raising=False)
+    monkeypatch.setattr(capi, "load", Recorder)
+    logits, labels = (None if t is None else t.as_subclass(_Cuda) for t in SLICES[name])
+    if name in REFUSED:
+        with pytest.raises(TypeError):
+            ops.logprobs(logits, labels)
+        assert not calls
+        return
+    lp, rank, entropy, _, _ = ops.logprobs(logits, labels)
+    assert entropy.shape == logits.shape[:-1] and entropy.is_contiguous()
+    assert labels is None or (lp.shape == rank.shape == labels.shape and lp.is_contiguous() and rank.is_contiguous())
+    (function, args), = calls
+    if function == "dabnn_logprobs":
+        at, kind, ld, lab, rows, classes = args[:6]
+        group_rows, ld_group, label_group = max(rows, 1), 0, 0
+    else:
+        assert function == "dabnn_logprobs_grouped"
+        at, kind, ld, ld_group, lab, label_group, group_rows, rows, classes = args[:9]
+    assert kind == 0 and classes == logits.shape[-1] and rows == logits.shape[:-1].numel()
+    read = [(at + 4 * (r // group_rows * ld_group + r % group_rows * ld)) for r in range(rows)]
+    index = [()] if logits.dim() == 1 else list(np.ndindex(*logits.shape[:-1]))
+    assert read == [logits[i].data_ptr() for i in index]
+    if labels is None:
+        assert lab is None
+    else:
+        assert [lab + 8 * (r // group_rows * label_group + r % group_rows) for r in range(rows)] == [labels[i].data_ptr() for i in index]
+    assert rows <= 1 or group_rows == 1 or ld >= classes
+
+
+def test_rows_with_a_pitch():
+    """Leading dimensions whose rows alone have a pitch are one matrix; others are refused."""
+    x = torch.zeros((3, 5, 40)).as_subclass(_Cuda)
+    assert ops._rows(x[..., 3:30], "x") == (15, 27, 40)
+    assert ops._rows(x[:, 2:3, :30], "x") == (3, 30, 200)
+    assert ops._rows(x[1:2, 1:3, :30], "x") == (2, 30, 40)
+    for bad in (x[:, 1:], x.transpose(0, 1), x[..., ::2], x.expand(2, 3, 5, 40)[:, :, 1:]):
+        with pytest.raises(TypeError):
+            ops._rows(bad, "x")
+
+
+def test_grouped_refusals(lib):
+    keep, p = buffer(4096)
+
+    def call(x=p, ld=100, ld_group=400, labels=p, label_group=3, group_rows=2, rows=4, lp=p, rank=p, top=0):
+        return lib.dabnn_logprobs_grouped(x, 0, ld, ld_group, labels, label_group, group_rows, rows, 100, lp, rank, p, None, None, top, None)
+
+    assert call(group_rows=0) == ARG and call(group_rows=-1) == ARG and call(rows=-1) == ARG
+    assert call(ld=99) == SHAPE
+    assert call(labels=None) == ARG and call(top=1) == ARG and call(x=None) == ARG
+    assert call(rows=0, x=None) == 0
