@@ -271,8 +271,8 @@ static int f8_gemm(Fp8Params p, const uint8_t* a, long long lda, const uint8_t* 
                       "fp8_gemm: cannot make a tensor map (no CUDA device, or a pitch beyond 2^40)");
     }
     CUtensorMap out_map{};
-    p.tma_out = 0;
-    if (nt > 64 && aligned_to(p.c, 16) && p.ldc * sizeof(T) % 16 == 0 && (unsigned long long)p.ldc * sizeof(T) < (1ull << 40) && p.N * sizeof(T) < INT_MAX) {
+    p.tma_out = 0;   // (a tensor store writes whole 16 bytes: rows that end inside them would have what lies behind them overwritten)
+    if (nt > 64 && aligned_to(p.c, 16) && p.ldc * sizeof(T) % 16 == 0 && p.N * sizeof(T) % 16 == 0 && (unsigned long long)p.ldc * sizeof(T) < (1ull << 40) && p.N * sizeof(T) < INT_MAX) {
         const unsigned long long dims[2] = {p.N * sizeof(T), (unsigned long long)p.M}, pitch[1] = {p.ldc * sizeof(T)};
         const unsigned box[2] = {128, 32};
         p.tma_out = make_u8_tensor_map(&out_map, static_cast<const unsigned char*>(p.c), 2, dims, pitch, box);

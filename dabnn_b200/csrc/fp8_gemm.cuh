@@ -44,7 +44,7 @@ struct Fp8Params {
     void* c;
     int M, N, nkb;                                     // activation rows, weight rows, blocks of K
     int tiles_n, ntiles;                               // tiles along the weight rows; all tiles
-    int tma_out;                                       // rows of c begin on 16-byte boundaries: tensor stores
+    int tma_out;                                       // rows of c begin and end on 16-byte boundaries: tensor stores
     int give_up_group, give_up_rank;                   // dabnn_debug_fp8_give_up: which group of factors of which CTA of a team is held to have run out of time; none: -1
 };
 

@@ -239,7 +239,8 @@ int dabnn_fp8_quantize(const void* in, int in_type, long long ld_in, uint8_t* ou
 /* c[i][j] = sum over blocks q of 128 along k of as(i, q) * bs(j / 128, q) * sum_{h in q} a[i][h] * b[j][h]  (+ bias[j]),
  * i < m, j < n: the product of activations [m][k] and weights [n][k], both e4m3, as dabnn_fp8_quantize writes them, with
  * as(i, q) = a_scales[i * as_row + q * as_block] and bs(j, q) = b_scales[j * bs_row + q * bs_block] of any fp32 value (the
- * two are multiplied first).  bias fp32 [n] or NULL; c of c_type, row pitch ldc, rounded once from the fp32 sum.  Rows of
+ * two are multiplied first).  bias fp32 [n] or NULL; c of c_type, row pitch ldc, rounded once from the fp32 sum; what lies
+ * between a row's end and its pitch is left as it was (n and ldc of whole 16 bytes are stored fastest).  Rows of
  * a and b begin on 16-byte boundaries (base and pitch), else DABNN_ERR_SHAPE. */
 int dabnn_fp8_gemm(const uint8_t* a, long long lda, const float* a_scales, long long as_row, long long as_block,
                    const uint8_t* b, long long ldb, const float* b_scales, long long bs_row, long long bs_block,

@@ -506,3 +506,31 @@ def test_collecting_the_code_of_a_wait_that_gave_up(ops):
     finally:
         capi.check(lib.dabnn_debug_fp8_give_up(-1, 0))
     assert ops.engine_status(collect=True) == 55 and ops.engine_status() == 0
+
+
+# ---------------------------------------------------------------------------------------------- paths of the product that other sizes do not reach
+@pytest.mark.parametrize("m,n,k", [(1, 40001, 300), (20, 50000, 144), (64, 60000, 640), (33, 80000, 200), (2, 39000, 1700), (7, 76100, 1), (16, 38000, 2050)])
+def test_gemm_few_rows_by_many_columns(ops, m, n, k):
+    """More tiles than CTAs of few rows at once: stages, accumulators and factors go on from one tile to the next, with counts of
+    blocks that are odd and no multiple of a group of factors."""
+    check_gemm(ops, m, n, k)
+
+
+@pytest.mark.parametrize("out", TYPES)
+@pytest.mark.parametrize("m,n", [(130, 2501), (300, 1003), (900, 1301), (1900, 2502)])
+def test_gemm_rows_that_end_inside_16_bytes(ops, m, n, out):
+    """An output whose pitch is a multiple of 16 bytes and whose rows are not: nothing behind a row or the last row is written."""
+    from dabnn_b200 import capi
+    k, dt = 200, TYPES[out]
+    a, sa, b, sb, bias = operands(m, n, k, 19)
+    if out == "f16":
+        sa, sb = sa * 2.0 ** -14, sb * 2.0 ** -6
+    c, tol = R.gemm(a, sa, b, sb, bias, torch.finfo(dt).eps)
+    ldc = (n + 15) // 16 * 16 + 16
+    store = torch.full((m + 3, ldc), -5.0, dtype=dt, device="cuda")
+    qa, qb, s, t, bv = R.f8(a), R.f8(b), dev(sa), dev(sb), dev(bias)
+    capi.check(capi.load().dabnn_fp8_gemm(qa.data_ptr(), qa.stride(0), s.data_ptr(), *s.stride(), qb.data_ptr(), qb.stride(0), t.data_ptr(), *t.stride(),
+                                          bv.data_ptr(), store.data_ptr(), {"f32": 0, "f16": 1, "bf16": 2}[out], ldc, m, n, k, ops._stream()))
+    R.close(values(store[:m, :n]), c, tol + (2.0 ** -25 if out == "f16" else 0.0))
+    store[:m, :n] = -5
+    assert (store == -5).all()

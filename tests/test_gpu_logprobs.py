@@ -358,3 +358,39 @@ def test_quantise_rows_with_a_pitch(ops):
     for part in (x[..., :300], x[..., 3:260], x[:, 2:3, 8:]):
         for a, b in zip(ops.fp8_quantize(part), ops.fp8_quantize(part.contiguous())):
             assert a.shape == b.shape and torch.equal(a.float(), b.float())
+
+
+@pytest.mark.parametrize("kind,classes", [("bf16", 9000), ("f32", 9000), ("f16", 20000)])
+def test_the_same_rows_alone_and_in_batches(ops, kind, classes):
+    """A row scored by a cluster, by a CTA and by a warp, as the number of rows has it: the same ranks and classes, log
+    probabilities and entropies within the bounds of each."""
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    x, labels = rows_of(16 * sms + 3, classes, 23, kind)
+    x[5] = torch.arange(classes, device="cuda") % 7                     # ties everywhere
+    lab = torch.tensor(labels).cuda()
+    full = ops.logprobs(x, lab, 20)                                     # a warp a row
+    (_, _, _, _, _), (tol, etol, ttol) = R.logprobs(x[:8].float().cpu().numpy(), np.array(labels[:8]), 20)
+    for rows in (1, 3, 8, sms, 4 * sms):                                # eight CTAs a row, fewer, one
+        part = ops.logprobs(x[:rows], lab[:rows], 20)
+        assert torch.equal(part[1], full[1][:rows]) and torch.equal(part[4], full[4][:rows])
+        n = min(rows, 8)
+        for got, all_of_it, bound in ((part[0], full[0], tol), (part[2], full[2], etol), (part[3], full[3], ttol)):
+            R.close(got[:n].cpu(), all_of_it[:n].cpu(), 2 * bound[:n])
+        for r in (rows - 1, rows // 2):                                 # and alone
+            one = ops.logprobs(x[r:r + 1], lab[r:r + 1], 20)
+            assert torch.equal(one[1], full[1][r:r + 1]) and torch.equal(one[4], full[4][r:r + 1])
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("classes", [40, 1000, 9000])
+def test_zeros_next_to_the_smallest_numbers(ops, classes, kind):
+    """Both zeros are one value, the smallest subnormals of the type on either side are others: as labels, before and behind."""
+    tiny = torch.finfo(TYPES[kind]).smallest_normal * torch.finfo(TYPES[kind]).eps
+    few = torch.tensor([0.0, tiny, -0.0, -tiny, 2 * tiny, -2 * tiny, 0.0, -0.0]).to(TYPES[kind])
+    assert few[1] > 0 and few[3] < 0 and (few.float()[1] / 2).to(TYPES[kind]) == 0
+    x = few[torch.randint(0, 8, (24, classes), generator=torch.Generator().manual_seed(classes))]
+    labels = [(i * classes) // 24 for i in range(24)]
+    for i in range(8):
+        x[3 * i, labels[3 * i]], x[3 * i + 1, labels[3 * i + 1]], x[3 * i + 2, labels[3 * i + 2]] = few[i], few[i], few[i]
+    check(ops, x.cuda(), labels, 7)
+    check(ops, x.cuda(), labels, 0)
