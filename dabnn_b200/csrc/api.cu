@@ -32,11 +32,17 @@ int sm_count() {
 typedef CUresult (*TensorMapEncode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                                     const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                     CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+// The encoders need an initialised driver and a current context.  Made by no call that a stream's capture forbids (cudaFree ends
+// one with an error): the first use may be inside it.
+static void make_context() {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) cudaGetLastError();
+}
 static TensorMapEncode tensor_map_encoder() {
     static TensorMapEncode encode = nullptr;
     static std::once_flag once;
     std::call_once(once, [] {
-        cudaFree(nullptr);   // the encoder needs an initialised driver and a current context
+        make_context();
         void* fn = nullptr;
         cudaDriverEntryPointQueryResult st;
         if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &st) == cudaSuccess &&
@@ -69,7 +75,7 @@ bool make_f32_im2col_map(CUtensorMap_st* map, const float* base, int n, int h, i
     static const TensorMapEncodeIm2col encode = [] {
         void* fn = nullptr;
         cudaDriverEntryPointQueryResult st;
-        cudaFree(nullptr);
+        make_context();
         if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeIm2col", &fn, 12000, cudaEnableDefault, &st) != cudaSuccess || st != cudaDriverEntryPointSuccess) {
             cudaGetLastError();
             fn = nullptr;

@@ -534,3 +534,46 @@ def test_gemm_rows_that_end_inside_16_bytes(ops, m, n, out):
     R.close(values(store[:m, :n]), c, tol + (2.0 ** -25 if out == "f16" else 0.0))
     store[:m, :n] = -5
     assert (store == -5).all()
+
+
+@pytest.mark.parametrize("first", ["head", "bytes", "floats"])
+def test_first_calls_of_a_process_inside_a_capture(first):
+    """Nothing has to be called before a capture: each kind of tile and of scoring is captured by the first call it ever has, and so are
+    the other kernels that load through tensor maps."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    program = """
+import torch
+from dabnn_b200 import ops
+g = torch.Generator(device="cuda").manual_seed(2)
+sets = []
+for m, n, k, c in ((1, 300, 300, 70), (1, 8192, 4096, 20000), (20, 700, 2048, 9000), (50, 600, 1280, 1000), (200, 4100, 512, 5000), (1000, 2600, 300, 300)):
+    x, w = torch.randn((m, k), device="cuda", generator=g), torch.randn((n, k), device="cuda", generator=g)
+    z = torch.randn((m, c), device="cuda", generator=g)
+    labels = torch.randint(0, c, (m,), device="cuda", generator=g)
+    sets.append((x, w, z, labels))
+x8, we = torch.randint(0, 2, (1, 16, 16, 64), dtype=torch.uint8, device="cuda"), torch.zeros(1 << 20, dtype=torch.uint8, device="cuda")
+image, weight = torch.randn((1, 16, 16, 64), device="cuda", generator=g), torch.randn((64, 3, 3, 64), device="cuda", generator=g)
+torch.cuda.synchronize()
+def run():
+    if FIRST == "bytes":
+        return [ops.bconv_u8_block(x8, we, 64, 3, 3, 1, 1, 1, 1)[0]]
+    if FIRST == "floats":
+        return [ops.fconv(image, weight, None, 1, 1, 1, 1)]
+    out = []
+    for x, w, z, labels in sets:
+        q, s = ops.fp8_quantize(x)
+        b, t = ops.fp8_quantize_weights(w)
+        out += [s, t, ops.fp8_gemm(q, s, b, t), ops.fp8_gemm(q, s, b, t, None, torch.bfloat16), *ops.logprobs(z, labels, 5), *ops.logprobs(z, labels, 0)[:3]]
+    return out
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    captured = run()
+graph.replay()
+for a, b in zip(captured, run()):
+    assert torch.equal(a, b)
+assert ops.engine_status() == 0
+"""
+    done = subprocess.run([sys.executable, "-c", f"FIRST = {first!r}\n" + program], cwd=Path(__file__).resolve().parent.parent, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stdout[-2000:] + done.stderr[-4000:]
