@@ -577,3 +577,20 @@ assert ops.engine_status() == 0
 """
     done = subprocess.run([sys.executable, "-c", f"FIRST = {first!r}\n" + program], cwd=Path(__file__).resolve().parent.parent, capture_output=True, text=True, timeout=300)
     assert done.returncode == 0, done.stdout[-2000:] + done.stderr[-4000:]
+
+
+@pytest.mark.parametrize("m", [2, 30, 60, 200, 900])
+@pytest.mark.parametrize("k", [1, 13, 100, 129, 257, 1100])
+def test_gemm_reads_nothing_behind_a_row(ops, m, k):
+    """Rows of a length that is no multiple of 16 bytes, NaN in all that lies behind them up to the pitch, behind the last row and
+    in front of the first."""
+    n = 2301
+    a, sa, b, sb, bias = operands(m, n, k, 29)
+    c, tol = R.gemm(a, sa, b, sb, bias, torch.finfo(torch.float32).eps)
+
+    def surrounded(v):
+        store = torch.full((v.shape[0] + 2, (k + 15) // 16 * 16), 0x7f, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+        store[1:-1, :k] = R.f8(v)
+        return store[1:-1, :k]
+
+    R.close(values(ops.fp8_gemm(surrounded(a), dev(sa), surrounded(b), dev(sb), dev(bias))), c, tol)
