@@ -135,6 +135,8 @@ class Net:
         shape = shape[:1] if shape[1:] == (1, 1) else shape
         lp = rank = tlp = ti = None
         if labels is not None:
+            if np.asarray(labels).dtype.kind not in "iu":
+                raise TypeError("logprobs: expected integer labels")
             labels = np.ascontiguousarray(labels, dtype=np.int64)
             if labels.shape != shape:
                 raise ValueError(f"logprobs: expected labels of shape {shape}")

@@ -394,3 +394,29 @@ def test_zeros_next_to_the_smallest_numbers(ops, classes, kind):
         x[3 * i, labels[3 * i]], x[3 * i + 1, labels[3 * i + 1]], x[3 * i + 2, labels[3 * i + 2]] = few[i], few[i], few[i]
     check(ops, x.cuda(), labels, 7)
     check(ops, x.cuda(), labels, 0)
+
+
+def test_net_logprobs_of_pixels(ops):
+    """A blob of several pixels an image: a row for each of them, labels and results in the blob's shape; labels that are no whole
+    numbers are refused."""
+    from dabnn_b200.bireal import OUTPUT_BLOB, build_bireal18
+    from dabnn_b200.dab_format import write_dab
+    from dabnn_b200.net import Net
+    rng = np.random.default_rng(1)
+    net = Net.create()
+    net.max_batch, net.optimize = 3, False
+    net.read_buf(write_dab(build_bireal18(image_hw=64, num_classes=10)))
+    for batch in (3, 2):
+        net.run(rng.normal(0, 1, (batch, 64, 64, 3)).astype(np.float32))
+        for name in ("s1b1_add_out", "s3b4_add_out"):
+            blob = net.get_blob(name)
+            assert blob.shape[0] == batch and blob.shape[1] > 1
+            labels = rng.integers(-1, blob.shape[3], blob.shape[:3])
+            want = ops.logprobs(torch.from_numpy(blob).cuda(), torch.from_numpy(labels).cuda(), 3)
+            for got, e in zip(net.logprobs(name, labels, 3), want):
+                np.testing.assert_array_equal(got, e.cpu().numpy())
+    for labels in ([0.0, 1.0], [True, False], ["1", "2"], [None, None]):
+        with pytest.raises(TypeError):
+            net.logprobs(OUTPUT_BLOB, labels)
+    np.testing.assert_array_equal(net.logprobs(OUTPUT_BLOB, [1, 2])[1], net.logprobs(OUTPUT_BLOB, np.array([1, 2], np.uint8))[1])
+    net.close()
