@@ -375,7 +375,7 @@ def _fp8_quantize(x, block_rows):
 
 def fp8_quantize(x):
     """Activations [..., K] (fp32, fp16, bf16) -> (e4m3 [..., K], fp32 scales [..., ceil(K / 128)]): one scale, a power of two,
-    for each 128 values of a row (see dabnn_fp8_quantize).  Rows of the result begin on 16-byte boundaries, as fp8_gemm wants
+    for each 128 values of a row (see dabnn_fp8_quantize).  The rows lie at equal steps.  Rows of the result begin on 16-byte boundaries, as fp8_gemm wants
     them; the scales lie block by block in memory."""
     q, scales = _fp8_quantize(x, 1)
     return (q, scales) if x.dim() == 2 else (q.unflatten(0, x.shape[:-1]), scales.unflatten(0, x.shape[:-1])) if x.dim() > 2 else (q[0], scales[0])
@@ -386,6 +386,16 @@ def fp8_quantize_weights(w):
     if w.dim() != 2:
         raise TypeError("fp8_quantize_weights: expected a matrix")
     return _fp8_quantize(w, FP8_BLOCK)
+
+
+def _byte_rows(t):
+    """[..., K] as a matrix; rows that do not lie at equal steps (a slice of a middle dimension) are copied, each to a 16-byte boundary."""
+    lead, k = t.shape[:-1], t.shape[-1]
+    if len(_levels(lead, t.stride()[:-1])) < 2 or t.is_contiguous():
+        return t.flatten(0, -2)
+    rows = torch.empty_strided((lead.numel(), k), ((k + 15) // 16 * 16, 1), dtype=t.dtype, device=t.device)
+    rows.unflatten(0, lead).copy_(t)
+    return rows
 
 
 def fp8_gemm(a, a_scales, b, b_scales, bias=None, out_dtype=torch.float32):
@@ -400,7 +410,7 @@ def fp8_gemm(a, a_scales, b, b_scales, bias=None, out_dtype=torch.float32):
     lead = None
     if a.dim() != 2:
         lead = a.shape[:-1]
-        a = a.unsqueeze(0) if a.dim() == 1 else a.flatten(0, -2)
+        a = a.unsqueeze(0) if a.dim() == 1 else _byte_rows(a)
         a_scales = a_scales.unsqueeze(0) if a_scales.dim() == 1 else a_scales.flatten(0, -2)
     if b.dim() != 2:
         raise TypeError("fp8_gemm: expected a matrix of weights")

@@ -594,3 +594,16 @@ def test_gemm_reads_nothing_behind_a_row(ops, m, k):
         return store[1:-1, :k]
 
     R.close(values(ops.fp8_gemm(surrounded(a), dev(sa), surrounded(b), dev(sb), dev(bias))), c, tol)
+
+
+@pytest.mark.parametrize("k", [100, 256])
+def test_gemm_of_slices_of_leading_dimensions(ops, k):
+    """Slices of every dimension of quantised activations, whose rows begin on 16-byte boundaries whether they lie at equal steps or not."""
+    g = torch.Generator().manual_seed(k)
+    q, s = ops.fp8_quantize(torch.randn((3, 5, 4, k), generator=g).cuda())
+    b, t = ops.fp8_quantize_weights(torch.randn((70, k), generator=g).cuda())
+    whole = ops.fp8_gemm(q, s, b, t)
+    for at in ((slice(None), slice(0, -1)), (slice(None), 2), (slice(None), slice(None), slice(1, 3)), (slice(1, 3), slice(1, 4), slice(0, 2)), (2, slice(1, 5, 2)),
+               (slice(None), slice(0, 0)), (0, 1, 2)):
+        assert torch.equal(ops.fp8_gemm(q[at], s[at], b, t), whole[at])
+    assert torch.equal(ops.fp8_gemm(q.transpose(0, 2), s.transpose(0, 2), b, t), whole.transpose(0, 2))
