@@ -470,14 +470,15 @@ def logprobs(logits, labels=None, top=0):
         raise TypeError("logprobs: expected fp32, fp16 or bf16")
     lead = logits.shape[:-1]
     lp = rank = tlp = ti = groups = None
-    if (logits.dim() == 2 or logits.is_contiguous()) and (labels is None or labels.is_contiguous()):
+    whole = labels is None or labels.is_contiguous()
+    if whole and (logits.dim() == 2 or logits.is_contiguous()):
         rows, classes, ld = _rows(logits, "logprobs")
     else:
         rows, classes, ld, *groups = _grouped_rows(logits, labels)
     if labels is not None:
         if labels.dtype != torch.int64 or labels.shape != lead:
             raise TypeError("logprobs: expected int64 labels, one for each row")
-        rank = torch.empty_like(labels, memory_format=torch.contiguous_format)
+        rank = torch.empty_like(labels) if whole else torch.empty_like(labels, memory_format=torch.contiguous_format)
         lp = torch.empty_like(rank, dtype=torch.float32)
         entropy = torch.empty_like(lp)
     else:
