@@ -17,8 +17,8 @@
 // epilogue that fetched its own waited for them, 8192 x 8192 x 4096 in 294 us), then the epilogue.
 //
 // What bounds it: at many rows the epilogue, whose trips to tensor memory take 735 cycles a block where the four instructions take
-// 512 (8192 x 8192 x 4096 231 us, 2.4 PFLOP/s; in long runs the power cap, 272 us), in tiles of 128 x 128 L2 (512 x 4096 x 4096
-// 14 us); at few rows HBM and set-up (1 x 16384 x 16384 54 us, 5.0 TB/s; 1 x 8192 x 4096 9.4 us, 3.6 TB/s).
+// 512 (8192 x 8192 x 4096 233 us, 2.4 PFLOP/s; in long runs the power cap, 277 us), in tiles of 128 x 128 L2 (512 x 4096 x 4096
+// 14 us); at few rows HBM and set-up (1 x 16384 x 16384 49 us, 5.5 TB/s; 1 x 8192 x 4096 9.5 us, 3.5 TB/s).
 //
 // Every wait on an mbarrier is bounded; one that gives up records a code (51 loader, 52 / 53 MMA warp waiting for an
 // accumulator / a stage, 54 epilogue, 55 factors) and raises the abort flag, in both CTAs of a pair, at which every role stops.
@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(Fp8Cfg<NT>::THREADS, Fp8Cfg<NT>::CTAS_PER_SM)
     };
     if (warp < Cfg::EPI_WARP0) {
         // a pair's 20 warps have 96 registers each at launch: these four give 32 of theirs to the epilogue's sixteen, whose sums and two
-        // chunks of an accumulator take 96
+        // chunks of an accumulator take 96 (with 16-bit results five values spill: 20 bytes stored, 40 loaded)
         if (PAIR) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
         if (warp == 0) {
             // =========================== TMA loads: one lane ===========================

@@ -16,7 +16,8 @@
 // A row is scored by one warp, or by a CTA of eight, or by a cluster of such CTAs where rows are few: the warps take the row's
 // batches in turn and their parts are joined at the end, lists of best classes by counting, for each entry, the better ones.
 //
-// What bounds it: issue and the pipe of ex2, 11 instructions for 32 logits; then HBM.  4096 rows of 65536 bf16, top 8: 124 us
+// What bounds it: with many rows the latency of a warp's steps (its batch from L2 first), of the pipes issue, 11 instructions for 32
+// logits, and ex2 most; then HBM.  4096 rows of 65536 bf16, top 8: 124 us
 // (4.3 TB/s; 101 us without alternatives); 4096 of 32768 fp32 without them 88 us (6.1 TB/s); 1 row of 131072, top 20: 12 us.
 #include <algorithm>
 #include <climits>
